@@ -205,8 +205,8 @@ def _module(s):
             s["module"] = loss.PolicyLoss(clip_low=0.2, clip_high=0.28, dual_clip=s["dual"] or None, kl_coef=0.04,
                                           entropy_coef=0.01, reduction=s["reduction"])
         else:
-            s["module"] = loss.PreferenceLoss(beta=0.1, kind=s["kind"], label_smoothing=s["smoothing"],
-                                              average=s["average"])
+            smoothing = s["smoothing"] if s["kind"] == "sigmoid" else 0.0        # the other kinds have none
+            s["module"] = loss.PreferenceLoss(beta=0.1, kind=s["kind"], label_smoothing=smoothing, average=s["average"])
     return s["module"]
 
 
