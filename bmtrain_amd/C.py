@@ -23,6 +23,7 @@ if not os.path.exists(LIBRARY_PATH):
 _lib = ctypes.CDLL(LIBRARY_PATH)
 
 _i64, _i32, _f, _p = ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
+_d = ctypes.c_double
 _HYPER = [_f] * 8  # beta1, beta2, eps, lr, scale, weight_decay, bias_correction1, bias_correction2
 
 # name -> argument types, in the order of include/bmt_hip.h
@@ -48,6 +49,14 @@ _SIGNATURES = {
     "grad_stats_noalloc_launcher": [_i64, _p, _i32, _p, _p, _p],
     "cross_entropy_reduce_forward_launcher": [_i64, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p],
     "cross_entropy_reduce_backward_launcher": [_i64, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p],
+    "token_logprobs_forward_launcher": [_i64] * 5 + [_p, _i32, _p, _i32, _i64, _f, _p, _p, _p, _p],
+    "token_logprobs_backward_launcher": [_i64] * 5 + [_p, _i32, _p, _i32, _i64, _f, _p, _p, _p, _p, _p],
+    "policy_loss_forward_launcher": [_i64, _i64, _i32] + [_p, _i64] * 5 + [_i32, _p, _i64, _d, _d, _d, _f, _f, _i32] + [_p] * 6,
+    "policy_loss_backward_launcher": [_i64, _i64, _i32, _i32, _p, _p, _p, _p, _i64, _f, _p, _p, _p],
+    "preference_loss_forward_launcher": [_i64, _i64, _i32] + [_p, _i64] * 3 + [_i32, _i32, _d, _d] + [_p] * 6,
+    "preference_loss_backward_launcher": [_i64, _i64, _i32, _p, _p, _p, _i64, _p, _p],
+    "grad_norm_multi_launcher": [_i32, _p, _i32, _d, _d, _d, _p, _p, _p],
+    "grad_scale_multi_launcher": [_i32, _p, _p, _i32, _p],
 }
 
 _lib.bmt_hip_last_error.restype = ctypes.c_char_p
@@ -92,6 +101,22 @@ _lib.grad_stats_workspace_floats.argtypes = [_i64]
 def grad_stats_workspace_floats(n: int) -> int:
     """Number of floats of device workspace grad_stats_*_launcher needs for n elements."""
     return int(_lib.grad_stats_workspace_floats(n))
+
+
+for _name, _argtypes in (("policy_loss_workspace_doubles", [_i64, _i64]), ("preference_loss_workspace_doubles", [_i64, _i64]),
+                         ("grad_norm_workspace_doubles", [_i32, _p])):
+    globals()[_name] = getattr(_lib, _name)
+    globals()[_name].restype = ctypes.c_int64
+    globals()[_name].argtypes = _argtypes
+
+
+def clip_table(rows):
+    """`bmt_clip_tensor` array of include/bmt_hip.h from (source pointer, destination pointer, n, source type code,
+    destination type code): four 64-bit words to an entry, the two 32-bit codes in the last.  Keep it alive over the call."""
+    words = []
+    for src, dst, n, src_type, dst_type in rows:
+        words += (src, dst, n, src_type | dst_type << 32)
+    return (_i64 * len(words))(*words)
 
 
 _lib.bmt_hip_flat_stream_stats.restype = ctypes.c_int
@@ -155,5 +180,7 @@ adam_fp16_multi_clip_launcher = _bind_multi("adam_fp16_multi_clip_launcher", 1)
 
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + ["is_bf16_supported", "bmt_hip_last_error", "grad_stats_workspace_floats",
                                                   "bmt_hip_flat_stream_stats", "grad_stats_multi_launcher",
+                                                  "policy_loss_workspace_doubles", "preference_loss_workspace_doubles",
+                                                  "grad_norm_workspace_doubles",
                                                   "adam_bf16_multi_launcher", "adam_fp16_multi_launcher",
                                                   "adam_bf16_multi_clip_launcher", "adam_fp16_multi_clip_launcher"])

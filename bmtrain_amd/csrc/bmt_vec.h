@@ -1,0 +1,138 @@
+// Device-side helpers of the kernels that take fp32, fp16 and bf16 alike: 16-byte vectors at any element alignment,
+// conversion to and from fp32, and the reductions they share.
+#pragma once
+#include "bmt_device.h"
+#include "bmt_host.h"
+#include <cstdio>
+
+namespace bmt {
+
+enum : int32_t { kFp32 = 0, kFp16 = 1, kBf16 = 2 };   // type codes of the C entries
+
+struct Single {};                                      // the fp32 tag beside Half and BFloat16
+
+// 16- / 8- / 4-byte accesses whose address is a multiple of the element size only.  gfx950 takes them in one
+// instruction; an access off its natural grid touches one more 128-byte line per wave.
+typedef u32x4 u32x4_any2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_any2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_any4 __attribute__((aligned(4)));
+
+// Bits: storage of one element; kVec: elements of a 16-byte vector.
+template <typename T>
+struct Elem {                                          // Half, BFloat16
+    typedef uint16_t Bits;
+    typedef u32x4_any2 Vec;
+    static constexpr int kVec = 8;
+    static __device__ __forceinline__ float get(Bits b) { return T::to_f32(b); }
+    static __device__ __forceinline__ Bits put(float f) { return T::from_f32(f); }
+    static __device__ __forceinline__ void unpack(const u32x4 &w, float *x) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[2 * k] = lo_f32<T>(w[k]), x[2 * k + 1] = hi_f32<T>(w[k]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *x) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = pack2<T>(x[2 * k], x[2 * k + 1]);
+        return w;
+    }
+};
+template <>
+struct Elem<Single> {
+    typedef uint32_t Bits;
+    typedef u32x4_any4 Vec;
+    static constexpr int kVec = 4;
+    static __device__ __forceinline__ float get(Bits b) { return __builtin_bit_cast(float, b); }
+    static __device__ __forceinline__ Bits put(float f) { return __builtin_bit_cast(uint32_t, f); }
+    static __device__ __forceinline__ void unpack(const u32x4 &w, float *x) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = get(w[k]);       // by value: a bit cast of w[k] itself reads element 0
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *x) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = put(x[k]);
+        return w;
+    }
+};
+
+// Elements in front of the first 16-byte boundary at or behind p, at most n.
+template <typename T>
+__device__ __forceinline__ int head_elements(const typename Elem<T>::Bits *p, int n) {
+    const int h = (int)((16u - ((uint32_t)(uintptr_t)p & 15u)) & 15u) / (int)sizeof(typename Elem<T>::Bits);
+    return h < n ? h : n;
+}
+
+// Four consecutive elements as floats (`count` of them exist; the others read as 0).
+template <typename T>
+__device__ __forceinline__ void load4(const typename Elem<T>::Bits *p, int count, float *x) {
+    if (count >= 4) {
+        if (sizeof(typename Elem<T>::Bits) == 2) {
+            const u32x2 w = *(const u32x2_any2 *)p;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                x[2 * k] = Elem<T>::get((typename Elem<T>::Bits)(w[k] & 0xFFFFu));
+                x[2 * k + 1] = Elem<T>::get((typename Elem<T>::Bits)(w[k] >> 16));
+            }
+        } else {
+            const u32x4 w = *(const u32x4_any4 *)p;
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = Elem<T>::get((typename Elem<T>::Bits)w[k]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = k < count ? Elem<T>::get(p[k]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(typename Elem<T>::Bits *p, int count, const float *x) {
+    if (count >= 4) {
+        if (sizeof(typename Elem<T>::Bits) == 2) {
+            u32x2 w;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                w[k] = (uint32_t)Elem<T>::put(x[2 * k]) | ((uint32_t)Elem<T>::put(x[2 * k + 1]) << 16);
+            *(u32x2_any2 *)p = w;
+        } else {
+            u32x4 w;
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = (uint32_t)Elem<T>::put(x[k]);
+            *(u32x4_any4 *)p = w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < count) p[k] = Elem<T>::put(x[k]);
+    }
+}
+// Four mask bytes as bits 0..3 (absent mask: all set); bytes behind `count` read as unset.
+typedef uint32_t u32_any1 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t mask4(const uint8_t *p, int count) {
+    if (!p) return count >= 4 ? 15u : (1u << count) - 1u;
+    uint32_t bits = 0;
+    if (count >= 4) {
+        const uint32_t w = *(const u32_any1 *)p;
+#pragma unroll
+        for (int k = 0; k < 4; k++) bits |= (w >> (8 * k) & 0xFFu) ? 1u << k : 0u;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < count && p[k]) bits |= 1u << k;
+    }
+    return bits;
+}
+
+// Sum over groups of `lanes` neighbouring lanes (a power of two up to 64); every lane ends with its group's sum.
+template <typename V>
+__device__ __forceinline__ V lanes_sum(V v, int lanes) {
+    for (int off = lanes >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+    return v;
+}
+
+// Host side: refuses a call of C entry `who` because of `why`.
+inline int refuse(const char *who, const char *why) {
+    char text[200];
+    snprintf(text, sizeof(text), "%s: %s", who, why);
+    return fail(-1, text);
+}
+
+}  // namespace bmt

@@ -1,0 +1,340 @@
+// Log-probabilities (and entropies) of given tokens under logits, and the logits' gradient, for gfx950.
+//
+// Row r of the logits holds x_0 .. x_{V-1}; with temperature T, z_j = (x_j - max x) / T and L = log sum_j e^{z_j}:
+//     logprob = z_target - L                 entropy H = L - (sum_j e^{z_j} z_j) / (sum_j e^{z_j})
+// and with upstream gradients g (of logprob) and h (of entropy), p_j = e^{z_j - L}:
+//     dx_j = ( g (1[j = target] - p_j) - h p_j (z_j - L + H) ) / T
+// The softmax is not stored: the forward pass reads the logits once and keeps {max, L, H} per row; the backward pass
+// reads the logits once more and writes the gradient.  Both are bound by HBM (2 or 4 bytes per element read, and as
+// many written on the way back).
+//
+// (x_j - max) is formed before it is scaled: it is exact for neighbouring values, so rows of large magnitude lose
+// nothing, and a row of the type's lowest value gives z = 0 instead of inf - inf.  All sums and exponents are fp32; the
+// gradient is rounded once, to the logits' type.
+//
+// A row is a workgroup's, or a wave's where rows are short.  Vectors are 16 bytes from the row's first 16-byte boundary,
+// the few elements in front of it and behind the last vector go one to a lane.
+#include "bmt_host.h"
+#include "bmt_vec.h"
+#include "../../include/bmt_hip.h"
+
+namespace bmt {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// z behind which e^z is 0 in fp32 (the smallest subnormal is e^-103.3): keeps 0 * -inf out of the entropy's sums
+constexpr float kFar = -1000.f;
+
+struct RowStats {       // what the backward pass needs of a row
+    float max, log_sum, entropy, unused;
+};
+
+struct LogitRows {      // row r starts at element (r / inner) * outer_stride + (r % inner) * inner_stride
+    const void *x;
+    int64_t outer_stride, inner_stride;
+    int32_t rows, inner, n;
+    __device__ __forceinline__ int64_t start(int32_t r) const {
+        if (inner >= rows) return (int64_t)r * inner_stride;
+        const int32_t o = r / inner;
+        return (int64_t)o * outer_stride + (int64_t)(r - o * inner) * inner_stride;
+    }
+};
+
+struct Targets {
+    const void *t;
+    int32_t is_64;
+    int64_t ignore;
+    __device__ __forceinline__ int64_t at(int32_t r) const {
+        return is_64 ? ((const int64_t *)t)[r] : (int64_t)((const int32_t *)t)[r];
+    }
+};
+
+// Running maximum m, s = sum 2^z and w = sum 2^z z with z = (x - m) * c in units of log 2.
+struct Online {
+    float m, s, w;
+};
+template <bool ENTROPY>
+__device__ __forceinline__ void online_join(Online &a, float m, float s, float w, float c) {
+    const float top = fmaxf(a.m, m);
+    const float da = (a.m - top) * c, db = (m - top) * c;
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+    if (ENTROPY) {      // the sums move by the shift of z: sum 2^(z+d) (z+d)
+        const float wa = __builtin_fmaf(fmaxf(da, kFar), a.s, a.w), wb = __builtin_fmaf(fmaxf(db, kFar), s, w);
+        a.w = wa * fa + wb * fb;
+    }
+    a.s = a.s * fa + s * fb;
+    a.m = top;
+}
+
+// K values x[0..K) into the running sums.
+template <bool ENTROPY, int K>
+__device__ __forceinline__ void online_add(Online &a, const float *x, float c) {
+    float top = x[0];
+#pragma unroll
+    for (int k = 1; k < K; k++) top = fmaxf(top, x[k]);
+    top = fmaxf(a.m, top);
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const float z = (x[k] - top) * c;
+        const float e = __builtin_amdgcn_exp2f(z);
+        s += e;
+        if (ENTROPY) w = __builtin_fmaf(e, fmaxf(z, kFar), w);
+    }
+    const float d = (a.m - top) * c;
+    const float f = __builtin_amdgcn_exp2f(d);
+    if (ENTROPY) a.w = __builtin_fmaf(__builtin_fmaf(fmaxf(d, kFar), a.s, a.w), f, w);
+    a.s = __builtin_fmaf(a.s, f, s);
+    a.m = top;
+}
+
+constexpr int kForwardUnroll = 4;
+
+// ROW: threads to a row (64: the workgroup's four waves take a row each).
+template <typename T, int ROW, bool ENTROPY>
+__global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
+    LogitRows in, Targets target, float inv_t, float *__restrict__ logprob, float *__restrict__ entropy,
+    RowStats *__restrict__ stats) {
+    typedef Elem<T> E;
+    constexpr int PER = ROW < 256 ? 256 / ROW : 1;      // rows of a workgroup
+    const int lane = threadIdx.x % ROW;
+    const int32_t r = (int32_t)(blockIdx.x * PER + threadIdx.x / ROW);
+    if (PER > 1 && r >= in.rows) return;
+    const int64_t t = target.at(r);
+    if (t == target.ignore) {
+        if (lane == 0) {
+            logprob[r] = 0.f;
+            if (ENTROPY) entropy[r] = 0.f;
+        }
+        return;
+    }
+    const typename E::Bits *x = (const typename E::Bits *)in.x + in.start(r);
+    const int n = in.n;
+    const int head = head_elements<T>(x, n);
+    const int nvec = (n - head) / E::kVec;
+    const u32x4 *body = (const u32x4 *)(x + head);
+    const float c = inv_t * kLog2e;
+    float xt = 0.f;
+    if (lane == 0 && (uint64_t)t < (uint64_t)n) xt = E::get(x[t]);
+
+    Online a = {-__FLT_MAX__, 0.f, 0.f};
+    constexpr int K = E::kVec;
+    int i = lane;
+    for (; i + (kForwardUnroll - 1) * ROW < nvec; i += kForwardUnroll * ROW) {
+        u32x4 w[kForwardUnroll];
+        float v[kForwardUnroll * K];
+#pragma unroll
+        for (int u = 0; u < kForwardUnroll; u++) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
+#pragma unroll
+        for (int u = 0; u < kForwardUnroll; u++) E::unpack(w[u], v + u * K);
+        online_add<ENTROPY, kForwardUnroll * K>(a, v, c);
+    }
+    for (; i < nvec; i += ROW) {
+        float v[K];
+        E::unpack(__builtin_nontemporal_load(body + i), v);
+        online_add<ENTROPY, K>(a, v, c);
+    }
+    const int tail_lo = head + nvec * K, edge = head + (n - tail_lo);      // fewer than 2 * kVec elements
+    if (lane < edge) {
+        const float v = E::get(x[lane < head ? lane : tail_lo + (lane - head)]);
+        online_add<ENTROPY, 1>(a, &v, c);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        online_join<ENTROPY>(a, __shfl_xor(a.m, off, kWave), __shfl_xor(a.s, off, kWave),
+                             ENTROPY ? __shfl_xor(a.w, off, kWave) : 0.f, c);
+    if (ROW > kWave) {
+        constexpr int WAVES = ROW / kWave > 0 ? ROW / kWave : 1;
+        __shared__ Online part[WAVES];
+        if (lane % kWave == 0) part[lane / kWave] = a;
+        __syncthreads();
+        if (lane != 0) return;
+        for (int k = 1; k < WAVES; k++) online_join<ENTROPY>(a, part[k].m, part[k].s, part[k].w, c);
+    }
+    if (lane == 0) {
+        const float log_sum = logf(a.s);
+        const float h = ENTROPY ? log_sum - kLn2 * (a.w / a.s) : 0.f;
+        logprob[r] = (uint64_t)t < (uint64_t)n ? (xt - a.m) * inv_t - log_sum : __builtin_nanf("");
+        if (ENTROPY) entropy[r] = h;
+        if (stats) stats[r] = RowStats{a.m, log_sum, h, 0.f};
+    }
+}
+
+constexpr int kBackwardUnroll = 4;
+
+template <typename T, int ROW, bool ENTROPY>
+__global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
+    LogitRows in, Targets target, float inv_t, const RowStats *__restrict__ stats, const float *__restrict__ grad_logprob,
+    const float *__restrict__ grad_entropy, typename Elem<T>::Bits *__restrict__ grad, int32_t tiles) {
+    typedef Elem<T> E;
+    constexpr int PER = 256 / ROW, K = E::kVec;
+    const int lane = threadIdx.x % ROW;
+    const uint32_t unit = blockIdx.x * PER + threadIdx.x / ROW;
+    const int32_t r = (int32_t)(unit / (uint32_t)tiles), tile = (int32_t)(unit - (uint32_t)r * (uint32_t)tiles);
+    if (PER > 1 && r >= in.rows) return;
+    const int64_t t = target.at(r);
+    const bool counted = t != target.ignore;
+    const float g = grad_logprob && counted ? grad_logprob[r] : 0.f;
+    const float h = ENTROPY && counted ? grad_entropy[r] : 0.f;
+    const bool live = !(g == 0.f && h == 0.f);          // nothing comes back through this row: its logits are not read
+    const typename E::Bits *x = (const typename E::Bits *)in.x + in.start(r);
+    typename E::Bits *d = grad + (int64_t)r * in.n;
+    const int n = in.n;
+    const int head = head_elements<T>(x, n);
+    const int nvec = (n - head) / K;
+    const u32x4 *body = (const u32x4 *)(x + head);
+    typename E::Vec *out = (typename E::Vec *)(d + head);
+    const RowStats st = live ? stats[r] : RowStats{0.f, 0.f, 0.f, 0.f};
+    const float a = -g * inv_t, b = -h * inv_t;
+    const float shift = st.entropy - st.log_sum;
+
+    auto one = [&](float v) {
+        const float z = (v - st.max) * inv_t;
+        const float p = __builtin_amdgcn_exp2f((z - st.log_sum) * kLog2e);
+        return p * (ENTROPY ? __builtin_fmaf(b, fmaxf(z, kFar) + shift, a) : a);
+    };
+    const int i0 = tile * (ROW * kBackwardUnroll) + lane;
+    u32x4 w[kBackwardUnroll];
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < kBackwardUnroll; u++)
+            if (i0 + u * ROW < nvec) w[u] = __builtin_nontemporal_load(body + i0 + u * ROW);
+    }
+#pragma unroll
+    for (int u = 0; u < kBackwardUnroll; u++) {
+        const int i = i0 + u * ROW;
+        if (i >= nvec) break;
+        u32x4 packed = {0u, 0u, 0u, 0u};
+        if (live) {
+            float v[K];
+            E::unpack(w[u], v);
+#pragma unroll
+            for (int k = 0; k < K; k++) v[k] = one(v[k]);
+            const int64_t at = t - (head + (int64_t)i * K);
+            if ((uint64_t)at < (uint64_t)K) {
+#pragma unroll
+                for (int k = 0; k < K; k++)
+                    if (k == (int)at) v[k] -= a;
+            }
+            packed = E::pack(v);
+        }
+        __builtin_nontemporal_store(packed, out + i);
+    }
+    const int tail_lo = head + nvec * K, edge = head + (n - tail_lo);
+    if (tile == 0 && lane < edge) {
+        const int j = lane < head ? lane : tail_lo + (lane - head);
+        float v = 0.f;
+        if (live) {
+            v = one(E::get(x[j]));
+            if (j == t) v -= a;
+        }
+        d[j] = E::put(v);
+    }
+}
+
+// Rows of up to this many elements go one to a wave: a workgroup's meeting point and its idle lanes cost more there.
+constexpr int32_t kWaveRow = 4096;
+
+static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void *x, int32_t type, const void *target, int32_t target_bits,
+                              float temperature) {
+    if (type != kFp32 && type != kFp16 && type != kBf16) return "unknown type code";
+    if (rows > 0x7FFFFFFF || n > 0x7FFFFFF0 || inner > 0x7FFFFFFF || inner < 1) return "too many rows or classes";
+    if (!x || !target) return "null pointer";
+    if ((uintptr_t)x % (type == kFp32 ? 4 : 2)) return "logits are not aligned to their elements";
+    if (target_bits != 32 && target_bits != 64) return "targets have 32 or 64 bits";
+    if ((uintptr_t)target % (uintptr_t)(target_bits / 8)) return "targets are not aligned to their elements";
+    if (!(temperature > 0.f) || !(1.f / temperature <= __FLT_MAX__) || !(temperature <= __FLT_MAX__))
+        return "temperature must be positive and finite";
+    return nullptr;
+}
+
+template <typename T, int ROW, bool ENTROPY>
+static void forward_launch(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+                           hipStream_t stream) {
+    constexpr int PER = ROW < 256 ? 256 / ROW : 1;
+    const unsigned grid = (unsigned)((in.rows + (int64_t)PER - 1) / PER);
+    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, ENTROPY>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
+                       logprob, entropy, stats);
+}
+template <typename T>
+static void forward_pick(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+                         hipStream_t stream) {
+    if (in.n <= kWaveRow) {
+        if (entropy) forward_launch<T, 64, true>(in, t, inv_t, logprob, entropy, stats, stream);
+        else forward_launch<T, 64, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    } else {
+        if (entropy) forward_launch<T, 256, true>(in, t, inv_t, logprob, entropy, stats, stream);
+        else forward_launch<T, 256, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    }
+}
+
+template <typename T, int ROW>
+static const char *backward_launch(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
+                                   const float *ge, void *grad, hipStream_t stream) {
+    const int64_t per_tile = (int64_t)ROW * kBackwardUnroll * Elem<T>::kVec;
+    const int64_t tiles = (in.n + per_tile - 1) / per_tile, per = 256 / ROW;
+    const int64_t grid = (in.rows * tiles + per - 1) / per;
+    if (in.rows * tiles > 0x7FFFFFFF) return "too many elements for one launch";
+    typedef typename Elem<T>::Bits Bits;
+    if (ge)
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, true>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+                           stats, gl, ge, (Bits *)grad, (int32_t)tiles);
+    else
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, false>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+                           stats, gl, ge, (Bits *)grad, (int32_t)tiles);
+    return nullptr;
+}
+template <typename T>
+static const char *backward_pick(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
+                                 const float *ge, void *grad, hipStream_t stream) {
+    return in.n <= kWaveRow ? backward_launch<T, 64>(in, t, inv_t, stats, gl, ge, grad, stream)
+                            : backward_launch<T, 256>(in, t, inv_t, stats, gl, ge, grad, stream);
+}
+
+}  // namespace bmt
+
+extern "C" int token_logprobs_forward_launcher(int64_t rows, int64_t n, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                                               const void *logits, int32_t type, const void *target, int32_t target_bits,
+                                               int64_t ignore_index, float temperature, void *logprob, void *entropy, void *stats,
+                                               void *stream) {
+    using namespace bmt;
+    if (rows <= 0 || n <= 0) return 0;
+    const char *who = "token_logprobs_forward_launcher";
+    if (const char *why = check_rows(rows, inner, n, logits, type, target, target_bits, temperature)) return refuse(who, why);
+    if (!logprob) return refuse(who, "null pointer");
+    if (((uintptr_t)logprob | (uintptr_t)entropy) % 4 || (uintptr_t)stats % 16) return refuse(who, "misaligned output");
+    const LogitRows in = {logits, outer_stride, inner_stride, (int32_t)rows, (int32_t)inner, (int32_t)n};
+    const Targets t = {target, target_bits == 64, ignore_index};
+    const float inv_t = 1.f / temperature;
+    hipStream_t s = (hipStream_t)stream;
+    if (type == kFp32) forward_pick<Single>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
+    else if (type == kFp16) forward_pick<Half>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
+    else forward_pick<BFloat16>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : fail((int)e, who, e);
+}
+
+extern "C" int token_logprobs_backward_launcher(int64_t rows, int64_t n, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                                                const void *logits, int32_t type, const void *target, int32_t target_bits,
+                                                int64_t ignore_index, float temperature, const void *stats,
+                                                const void *grad_logprob, const void *grad_entropy, void *grad, void *stream) {
+    using namespace bmt;
+    if (rows <= 0 || n <= 0) return 0;
+    const char *who = "token_logprobs_backward_launcher";
+    if (const char *why = check_rows(rows, inner, n, logits, type, target, target_bits, temperature)) return refuse(who, why);
+    if (!stats || !grad) return refuse(who, "null pointer");
+    if (((uintptr_t)grad_logprob | (uintptr_t)grad_entropy) % 4 || (uintptr_t)stats % 16 || (uintptr_t)grad % (type == kFp32 ? 4 : 2))
+        return refuse(who, "misaligned pointer");
+    const LogitRows in = {logits, outer_stride, inner_stride, (int32_t)rows, (int32_t)inner, (int32_t)n};
+    const Targets t = {target, target_bits == 64, ignore_index};
+    const float inv_t = 1.f / temperature;
+    const RowStats *st = (const RowStats *)stats;
+    const float *gl = (const float *)grad_logprob, *ge = (const float *)grad_entropy;
+    hipStream_t s = (hipStream_t)stream;
+    const char *why = type == kFp32   ? backward_pick<Single>(in, t, inv_t, st, gl, ge, grad, s)
+                      : type == kFp16 ? backward_pick<Half>(in, t, inv_t, st, gl, ge, grad, s)
+                                      : backward_pick<BFloat16>(in, t, inv_t, st, gl, ge, grad, s);
+    if (why) return refuse(who, why);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : fail((int)e, who, e);
+}

@@ -205,3 +205,51 @@ def adam_multi(tensors, beta1: float, beta2: float, eps: float, lr: float, scale
         launcher = C.adam_bf16_multi_clip_launcher if flavour == torch.bfloat16 else C.adam_fp16_multi_clip_launcher
         launcher(rows, beta1, beta2, eps, lr, scale, weight_decay, bias_correction1, bias_correction2, grad_coef,
                  _current_stream())
+
+
+_TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def clip_rows(grads, outs=None):
+    """Entries (source, destination, n, type codes) of ``C.clip_table`` for dense GPU tensors of fp32, fp16 or bf16 on one
+    device; ``outs`` (default: the gradients themselves) have their gradients' shapes and strides."""
+    rows = []
+    device = grads[0].device if grads else None
+    for g, o in zip(grads, grads if outs is None else outs):
+        if g.dtype not in _TYPE_CODES or o.dtype not in _TYPE_CODES:
+            raise ValueError(f"gradients must be fp32, fp16 or bf16, not {g.dtype} to {o.dtype}")
+        assert g.is_cuda and g.device == device and o.device == device, "gradients must be on one cuda device"
+        if not g.is_contiguous() or (o is not g and not o.is_contiguous()):
+            assert is_dense(g), "gradients must not have gaps nor elements that share memory"
+            assert o.stride() == g.stride(), "outputs must have their gradients' strides"
+        assert o.shape == g.shape, "outputs must have their gradients' shapes"
+        rows.append((g.data_ptr(), o.data_ptr(), g.numel(), _TYPE_CODES[g.dtype], _TYPE_CODES[o.dtype]))
+    return rows
+
+
+def is_dense(t: torch.Tensor) -> bool:
+    """True if the elements of `t` fill one run of memory without gaps, in whatever order of dimensions."""
+    expected = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
+        if stride != expected:
+            return t.numel() == 0
+        expected *= size
+    return True
+
+
+def grad_norm_multi(rows, use_max: bool, max_norm: float, eps: float, scale: float, out: torch.Tensor) -> None:
+    """``out[0] = n / scale`` and the clipping factor ``out[1] = max_norm * scale / (n + eps)`` for n the L2 norm (or the
+    largest magnitude) over the gradients of ``rows`` (``clip_rows``); ``out`` is two floats."""
+    assert out.is_cuda and out.dtype == torch.float32 and out.numel() == 2 and out.is_contiguous()
+    table = C.clip_table(rows)
+    workspace = torch.empty(C.grad_norm_workspace_doubles(len(rows), table), dtype=torch.float64, device=out.device)
+    C.grad_norm_multi_launcher(len(rows), table, int(use_max), max_norm, eps, scale, workspace.data_ptr(), out.data_ptr(),
+                               _current_stream())
+
+
+def grad_scale_multi(rows, coef: torch.Tensor, round_coef: bool = False) -> None:
+    """Every destination of ``rows`` = its source times ``coef`` (one float on the GPU) if that is below one, else the
+    source itself; ``round_coef``: times the factor rounded to the source's type."""
+    assert coef.is_cuda and coef.dtype == torch.float32 and coef.numel() == 1, "coef must be one float on cuda"
+    if rows:
+        C.grad_scale_multi_launcher(len(rows), C.clip_table(rows), coef.data_ptr(), int(round_coef), _current_stream())

@@ -1,0 +1,57 @@
+"""Global norm and clipping over a list of gradients without a host read; for programs that step their gradients
+without :class:`OptimManager` (whose ``clip_grad_norm`` uses the same scaling kernel), or keep fp32 accumulators
+(bmtrain/optim/optim_manager.py:158-200 is the reference's clipping)."""
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from . import _function as F
+
+
+@torch.no_grad()
+def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, eps: float = 1e-6, scale: float = 1.0,
+               out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    r"""Clips ``grads`` to the global norm ``max_norm`` and returns their norm before clipping, a 0-dim fp32 tensor on
+    their device:
+
+    .. math::
+        n = \Big(\sum_k \sum_i g_{k,i}^2\Big)^{1/2} \text{ or } \max |g_{k,i}|, \qquad
+        c = \frac{\text{max\_norm} \cdot \text{scale}}{n + \text{eps}}, \qquad
+        \text{out} = c < 1\ ?\ c\, g : g
+
+    Args:
+        grads: fp32, fp16 and bf16 tensors on one GPU, in any mixture; each dense (contiguous in some order of its dimensions).
+        max_norm: the largest norm of the unscaled gradients.
+        norm_type: 2.0, or ``math.inf`` / ``'inf'`` for the largest magnitude.
+        scale: the loss scale the gradients carry; the returned norm is divided by it.
+        out: tensors of the gradients' shapes (and strides, where not contiguous), of any of the three types, that
+            receive the clipped gradients - fp32 accumulators into the 16-bit gradients of an optimizer, say; ``None``
+            clips in place.  An output may be its own gradient but share memory with nothing else of the call
+            (``RuntimeError``; the gradients themselves are not listed twice either when they are clipped in place).
+
+    Nothing is read by the host, so the call can be captured into a graph.  Squares are summed in 64 bits in a fixed
+    order, the product with the factor is fp32 and rounded to the output's type once.  With an infinite norm the factor
+    is 0 (infinities turn into NaN); a NaN norm leaves the gradients as they are.  Gradients of ``None`` are skipped,
+    together with their output.
+    """
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(grads)} gradients but {len(outs)} outputs")
+    if any(g is None for g in grads):
+        outs = [o for g, o in zip(grads, outs) if g is not None]
+        grads = [g for g in grads if g is not None]
+    if not (max_norm >= 0 and eps >= 0 and scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"max_norm and eps must not be negative and scale must be positive: {max_norm}, {eps}, {scale}")
+    use_max = norm_type in ("inf", math.inf)
+    if not use_max and norm_type != 2:
+        raise ValueError(f"norm_type must be 2 or inf, not {norm_type}")
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device="cuda" if torch.cuda.is_available() else "cpu")
+    rows = F.clip_rows(grads, outs)
+    with torch.cuda.device(grads[0].device):
+        result = torch.empty(2, dtype=torch.float32, device=grads[0].device)
+        F.grad_norm_multi(rows, use_max, float(max_norm), float(eps), float(scale), result)
+        F.grad_scale_multi(rows, result[1])
+    return result[0]

@@ -274,6 +274,96 @@ BMT_API int grad_stats_multi_launcher(int32_t count, const bmt_scan_tensor *tens
                                       void *flag, void *workspace, void *stream);
 
 /*
+ * The entries below have no counterpart in the reference's extension: what preference and policy tuning need between
+ * the logits and the optimizer.  `type` is 0 = fp32, 1 = fp16, 2 = bf16.  Strides count elements.  Pointers are aligned to
+ * their elements (doubles to 8 bytes, `stats` of the token log-probabilities to 16); nothing more is asked.
+ */
+
+/*
+ * token_logprobs_{forward,backward}_launcher.  Row r of `rows` rows of n logits starts at element
+ * (r / inner) * outer_stride + (r % inner) * inner_stride (a [batch, time, n] view: inner = time); inner >= rows leaves
+ * the inner stride alone.  target: int32 or int64 (target_bits) per row.  With temperature T > 0,
+ * z_j = (x_j - max x) / T and L = log sum_j e^z_j:
+ *   logprob[r] = z_target - L;   entropy[r] = L - sum_j e^z_j z_j / sum_j e^z_j   (fp32; entropy may be NULL)
+ *   stats: float[4 * rows] for the backward call, or NULL;
+ *   grad[r, j] = (g (1[j == target] - p_j) - h p_j (log p_j + entropy[r])) / T,  p_j = e^(z_j - L), contiguous [rows, n]
+ * with g = grad_logprob[r], h = grad_entropy[r] (fp32; either may be NULL for zeros).
+ * A row whose target is ignore_index has results 0 and a gradient row of 0, and its logits are not read; a row with
+ * g == h == 0 has a gradient row of 0 and is not read on the way back.  Another target outside [0, n): logprob NaN, and
+ * a gradient without the one-hot term.
+ */
+BMT_API int token_logprobs_forward_launcher(int64_t rows, int64_t n, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                                            const void *logits, int32_t type, const void *target, int32_t target_bits,
+                                            int64_t ignore_index, float temperature, void *logprob, void *entropy, void *stats,
+                                            void *stream);
+BMT_API int token_logprobs_backward_launcher(int64_t rows, int64_t n, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                                             const void *logits, int32_t type, const void *target, int32_t target_bits,
+                                             int64_t ignore_index, float temperature, const void *stats,
+                                             const void *grad_logprob, const void *grad_entropy, void *grad, void *stream);
+
+/*
+ * policy_loss_{forward,backward}_launcher: rows sequences of `time` tokens, each array with its own row stride and its
+ * tokens next to each other.  Per token under the mask (uint8, NULL = all), d = logprob - old, r = e^d, q = ref - logprob:
+ *   policy = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), and at most -dual_clip A where A < 0 (dual_clip 0: none)
+ *   kl = e^q - 1 - q (0 without ref),   old_kl = e^d - 1 - d
+ *   loss = R(policy) + kl_coef R(kl) - entropy_coef R(entropy);   stats[5] = R of policy, kl, entropy, clipped, old_kl
+ * reduction 0: mean over the tokens under the mask; 1: mean over the sequences with tokens of their means; 2: sum.
+ * Nothing under the mask: 0.  advantage: float, one per row (advantage_col 0) or per token (1).
+ * saved: float[rows * time] (the derivative before its weight) or NULL when no backward call follows; weights:
+ * float[1 + rows] (float[1] unless reduction is 1); workspace: double[policy_loss_workspace_doubles(rows, time)].
+ * backward: grad_logprob = saved * weight * upstream[0]; grad_entropy = -entropy_coef * weight * upstream[0] under the
+ * mask; both contiguous, of `type`, either may be NULL.
+ */
+BMT_API int64_t policy_loss_workspace_doubles(int64_t rows, int64_t time);
+BMT_API int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t type, const void *logprob, int64_t logprob_row,
+                                         const void *old_logprob, int64_t old_row, const void *ref_logprob, int64_t ref_row,
+                                         const void *entropy, int64_t entropy_row, const void *advantage, int64_t advantage_row,
+                                         int32_t advantage_col, const void *mask, int64_t mask_row, double clip_low,
+                                         double clip_high, double dual_clip, float kl_coef, float entropy_coef,
+                                         int32_t reduction, void *saved, void *weights, void *workspace, void *loss, void *stats,
+                                         void *stream);
+BMT_API int policy_loss_backward_launcher(int64_t rows, int64_t time, int32_t type, int32_t reduction, const void *saved,
+                                          const void *weights, const void *upstream, const void *mask, int64_t mask_row,
+                                          float entropy_coef, void *grad_logprob, void *grad_entropy, void *stream);
+
+/*
+ * preference_loss_{forward,backward}_launcher: rows 0 .. pairs-1 hold the chosen answers' token log-probabilities, rows
+ * pairs .. 2 pairs-1 the rejected ones'.  s = sum over the mask of logprob - ref (ref NULL: 0), divided by the row's
+ * token count when `average`; h = s_chosen - s_rejected, x = beta h:
+ *   kind 0: -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x);  1: (h - 1/(2 beta))^2;  2: max(0, 1 - x)
+ *   loss = mean over the pairs with a token in either row (none: 0);  chosen / rejected[pairs] = beta s
+ * slope: float[1 + 2 pairs] for the backward call; workspace: double[preference_loss_workspace_doubles(pairs, time)].
+ */
+BMT_API int64_t preference_loss_workspace_doubles(int64_t pairs, int64_t time);
+BMT_API int preference_loss_forward_launcher(int64_t pairs, int64_t time, int32_t type, const void *logprob, int64_t logprob_row,
+                                             const void *ref_logprob, int64_t ref_row, const void *mask, int64_t mask_row,
+                                             int32_t kind, int32_t average, double beta, double label_smoothing, void *workspace,
+                                             void *loss, void *chosen, void *rejected, void *slope, void *stream);
+BMT_API int preference_loss_backward_launcher(int64_t pairs, int64_t time, int32_t type, const void *slope, const void *upstream,
+                                              const void *mask, int64_t mask_row, void *grad_logprob, void *stream);
+
+/*
+ * grad_norm_multi_launcher / grad_scale_multi_launcher — the norm and the scaling of clip_grad_norm
+ * (bmtrain/optim/optim_manager.py:158-200) over a list of tensors of mixed types in a few launches, without a host read.
+ *   norm:  n = sqrt(sum g^2) over all tensors (use_max: max |g|); out[0] = n / scale, out[1] = max_norm * scale / (n + eps)
+ *   scale: c = coef[0]; dst = src * c where c < 1, otherwise dst = src (NaN included); round_coef: c is first rounded
+ *          to the tensor's src type.  dst may be src itself (same type); any other sharing of memory is refused.
+ * `tensors` is a host array, checked before the first launch; entries with n <= 0 are skipped; dst is not looked at by the
+ * norm.  workspace: double[grad_norm_workspace_doubles(count, tensors)].  Equal inputs give equal bits.
+ */
+typedef struct bmt_clip_tensor {
+    const void *src;
+    void *dst;
+    int64_t n;
+    int32_t src_type, dst_type;
+} bmt_clip_tensor;
+BMT_API int64_t grad_norm_workspace_doubles(int32_t count, const bmt_clip_tensor *tensors);
+BMT_API int grad_norm_multi_launcher(int32_t count, const bmt_clip_tensor *tensors, int32_t use_max, double max_norm, double eps,
+                                     double scale, void *workspace, void *out, void *stream);
+BMT_API int grad_scale_multi_launcher(int32_t count, const bmt_clip_tensor *tensors, const void *coef, int32_t round_coef,
+                                      void *stream);
+
+/*
  * bmt_hip_flat_stream_stats — diagnostics, no counterpart in the reference.  For the current device, since the
  * library was loaded: out[0] = launches of the in-place cross-entropy / softmax kernels that ran as the resident
  * ticket-ordered grid, out[1] = large launches that could not get ticket counters (stream under capture,
