@@ -8,6 +8,7 @@ top of the C ABI of ``libbmt_hip.so`` (include/bmt_hip.h), loaded with ctypes.
 There is no fallback: if the shared library has not been built, importing this
 module raises ImportError; a non-zero status from a launcher raises RuntimeError.
 """
+import array
 import ctypes
 import os
 
@@ -110,13 +111,15 @@ for _name, _argtypes in (("policy_loss_workspace_doubles", [_i64, _i64]), ("pref
     globals()[_name].argtypes = _argtypes
 
 
-def clip_table(rows):
-    """`bmt_clip_tensor` array of include/bmt_hip.h from (source pointer, destination pointer, n, source type code,
-    destination type code): four 64-bit words to an entry, the two 32-bit codes in the last.  Keep it alive over the call."""
-    words = []
-    for src, dst, n, src_type, dst_type in rows:
-        words += (src, dst, n, src_type | dst_type << 32)
-    return (_i64 * len(words))(*words)
+def clip_table(sources, destinations, counts, source_types, destination_types):
+    """`bmt_clip_tensor` array of include/bmt_hip.h from parallel lists of pointers, element counts and type codes: four
+    64-bit words to an entry, the two 32-bit codes in the last.  Its address is `buffer_info()[0]`; keep it over the call."""
+    words = [0] * (4 * len(sources))
+    words[0::4] = sources
+    words[1::4] = destinations
+    words[2::4] = counts
+    words[3::4] = [s | d << 32 for s, d in zip(source_types, destination_types)]
+    return array.array("q", words)
 
 
 _lib.bmt_hip_flat_stream_stats.restype = ctypes.c_int

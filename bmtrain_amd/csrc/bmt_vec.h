@@ -104,21 +104,83 @@ __device__ __forceinline__ void store4(typename Elem<T>::Bits *p, int count, con
             if (k < count) p[k] = Elem<T>::put(x[k]);
     }
 }
-// Four mask bytes as bits 0..3 (absent mask: all set); bytes behind `count` read as unset.
-typedef uint32_t u32_any1 __attribute__((aligned(1)));
-__device__ __forceinline__ uint32_t mask4(const uint8_t *p, int count) {
-    if (!p) return count >= 4 ? 15u : (1u << count) - 1u;
-    uint32_t bits = 0;
-    if (count >= 4) {
-        const uint32_t w = *(const u32_any1 *)p;
+// Four consecutive elements as raw bits, to be converted later: loads of several arrays can be on their way before the
+// first value is needed.  load: all four exist; load_some: the first `count` do, the others read as 0.
+template <typename T>
+struct Raw4 {
+    uint32_t w[sizeof(typename Elem<T>::Bits)];        // 2 dwords of 16-bit elements, 4 of 32-bit ones
+    __device__ __forceinline__ void load(const typename Elem<T>::Bits *p) {
+        if (sizeof(typename Elem<T>::Bits) == 2) {
+            const u32x2 v = *(const u32x2_any2 *)p;
+            w[0] = v[0], w[1] = v[1];
+        } else {
+            const u32x4 v = *(const u32x4_any4 *)p;
 #pragma unroll
-        for (int k = 0; k < 4; k++) bits |= (w >> (8 * k) & 0xFFu) ? 1u << k : 0u;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (k < count && p[k]) bits |= 1u << k;
+            for (int k = 0; k < (int)sizeof(typename Elem<T>::Bits); k++) w[k] = v[k];
+        }
     }
-    return bits;
+    __device__ __forceinline__ void load_some(const typename Elem<T>::Bits *p, int count) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const typename Elem<T>::Bits b = k < count ? p[k] : 0;
+            if (sizeof(b) == 4) w[k] = b;
+            else w[k / 2] = k % 2 ? (w[k / 2] & 0xFFFFu) | ((uint32_t)b << 16) : (uint32_t)b;
+        }
+    }
+    __device__ __forceinline__ float get(int k) const {
+        if (sizeof(typename Elem<T>::Bits) == 4) return Elem<T>::get((typename Elem<T>::Bits)w[k]);
+        return Elem<T>::get((typename Elem<T>::Bits)(w[k / 2] >> (16 * (k % 2))));
+    }
+};
+
+// Four mask bytes, one to each byte of a dword (absent mask: all set); bytes behind `count` read as unset.
+typedef uint32_t u32_any1 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t load_mask4(const uint8_t *p, int count) {
+    if (!p) return count >= 4 ? 0x01010101u : 0x01010101u >> (8 * (4 - count));
+    if (count >= 4) return *(const u32_any1 *)p;
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (k < count) w |= (uint32_t)p[k] << (8 * k);
+    return w;
+}
+__device__ __forceinline__ bool mask_set(uint32_t w, int k) { return (w >> (8 * k) & 0xFFu) != 0; }
+__device__ __forceinline__ int mask_count(uint32_t w) {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) n += mask_set(w, k) ? 1 : 0;
+    return n;
+}
+
+// Sums of eight values over a wave: lane 8 j ends with the sum of v[j].  Every step halves the values a lane carries
+// (it hands one half to its partner and takes the other), so eight values cost ten exchanges instead of 48.
+template <typename V>
+__device__ __forceinline__ V wave_sum8(V *v) {
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int half = 4; half > 0; half >>= 1) {
+        const bool upper = (lane & (8 * half)) != 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j >= half) break;
+            const V keep = upper ? v[j + half] : v[j], give = upper ? v[j] : v[j + half];
+            v[j] = keep + __shfl_xor(give, 8 * half, kWave);
+        }
+    }
+    V sum = v[0];
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+    return sum;
+}
+
+// Workgroups are dealt to the eight XCDs in turn.  This numbering gives every XCD runs of RUN consecutive units of work
+// instead (the last incomplete round of 8 * RUN units keeps the plain order), so that what one XCD's L2 and its share of
+// the memory channels see is consecutive.
+template <uint32_t RUN>
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t count) {
+    constexpr uint32_t kXcds = 8, kRound = kXcds * RUN;
+    const uint32_t base = id / kRound * kRound, k = id - base;
+    return base + kRound <= count ? base + (k % kXcds) * RUN + k / kXcds : id;
 }
 
 // Sum over groups of `lanes` neighbouring lanes (a power of two up to 64); every lane ends with its group's sum.

@@ -11,8 +11,12 @@
 // Squares are formed and added in 64 bits: an fp32 or bf16 gradient's square may lie outside fp32's range.  Partial
 // sums, one to a tile, are added in a fixed order: equal inputs give equal bits.
 // Up to kBatch tensors of one pair of types travel in a launch's arguments; tiles are numbered through the tensors and
-// a workgroup finds its tensor there.  The second pass takes the tiles in the opposite order: what the first one read
-// last is still in the last-level cache.
+// a workgroup finds its tensor there.  The second pass goes through the gradients backwards, from what the first one
+// read last, and both read and write past the caches (non-temporal).
+// Measured on 45 fp32 tensors of 1.01 B elements into bf16: norm 0.59 ms (6.9 TB/s; 0.66 ms with temporal loads, 0.66
+// with half the tile), scaling 0.91 ms (6.7 TB/s; 0.95 with one tile to an XCD in turn, 0.98 with three vectors to a
+// lane); 202 M bf16 elements 64 + 128 us.  Leaving the first pass's last 128 to 240 MiB to the cache changed nothing, runs
+// of tiles on one XCD made the norm pass slower (0.61 ms).
 #include "bmt_vec.h"
 #include "../../include/bmt_hip.h"
 
@@ -23,8 +27,11 @@
 namespace bmt {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kUnroll = 4;               // vectors of a lane: a tile is 64 KiB of the input
+constexpr int kThreads = 1024;           // norm pass: a tile is 8 vectors of 1,024 lanes, 128 KiB
+constexpr int kUnroll = 8;
+constexpr int kScaleThreads = 256;       // scaling pass: 2 vectors of 256 lanes, 8 KiB
+constexpr int kScaleUnroll = 2;
+constexpr uint32_t kScaleRun = 256;      // workgroups of consecutive tiles on one XCD
 constexpr int kBatch = 96;
 
 struct Batch {
@@ -33,9 +40,6 @@ struct Batch {
     int64_t n[kBatch];
     uint32_t first[kBatch];              // number of a tensor's first tile; 0xFFFFFFFF behind the last tensor
 };
-
-template <typename T>
-constexpr int64_t tile_elements() { return (int64_t)kThreads * kUnroll * Elem<T>::kVec; }
 
 // The tensor of tile `tile`: the last one that starts at or in front of it (a bisection over the arguments).
 __device__ __forceinline__ int find_tensor(const Batch &b, uint32_t tile) {
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(Batch batch, double
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
         w[u] = u32x4{0u, 0u, 0u, 0u};
-        if (i0 + u * kThreads < nvec) w[u] = body[i0 + u * kThreads];
+        if (i0 + u * kThreads < nvec) w[u] = __builtin_nontemporal_load(body + i0 + u * kThreads);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
@@ -136,45 +140,54 @@ __global__ __launch_bounds__(kThreads) void grad_norm_finish_kernel(const double
     }
 }
 
+// K elements of type D, 8 or 16 bytes at a time, not kept in the cache.
+template <typename D, int K>
+__device__ __forceinline__ void store_past_cache(typename Elem<D>::Bits *to, const float *x) {
+    if (sizeof(typename Elem<D>::Bits) * K == 8) {
+        u32x2 w;
+        w[0] = (uint32_t)Elem<D>::put(x[0]) | ((uint32_t)Elem<D>::put(x[1]) << 16);
+        w[1] = (uint32_t)Elem<D>::put(x[2]) | ((uint32_t)Elem<D>::put(x[3]) << 16);
+        __builtin_nontemporal_store(w, (u32x2_any2 *)to);
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; k += Elem<D>::kVec) __builtin_nontemporal_store(Elem<D>::pack(x + k), (typename Elem<D>::Vec *)(to + k));
+    }
+}
+
 // The factor a tensor is multiplied by: c, or c rounded to the tensor's type (what torch's multiplication of a 16-bit
 // tensor by a 0-dim fp32 tensor does); 1 where c is not below 1, a NaN among them.
 template <typename S, typename D>
-__global__ __launch_bounds__(kThreads) void grad_scale_kernel(Batch batch, const float *__restrict__ coef, int32_t round_coef) {
+__global__ __launch_bounds__(kScaleThreads) void grad_scale_kernel(Batch batch, const float *__restrict__ coef, int32_t round_coef) {
     typedef Elem<S> E;
     constexpr int K = E::kVec;
     const float c = coef[0];
     const bool scales = c < 1.f;
-    const uint32_t number = gridDim.x - 1 - blockIdx.x;
+    const uint32_t number = xcd_run<kScaleRun>(blockIdx.x, gridDim.x);
     const int which = find_tensor(batch, number);
     const typename E::Bits *g = (const typename E::Bits *)batch.src[which];
     typename Elem<D>::Bits *o = (typename Elem<D>::Bits *)batch.dst[which];
     if (!scales && (const void *)g == (const void *)o) return;
     const float f = !scales ? 1.f : round_coef ? E::get(E::put(c)) : c;
     const int64_t n = batch.n[which];
-    const uint32_t tile = number - batch.first[which];
+    constexpr int64_t kTile = (int64_t)kScaleThreads * kScaleUnroll;       // vectors
+    const int64_t tile = (n + kTile * K - 1) / (kTile * K) - 1 - (number - batch.first[which]);      // last tile first
     const int head = head_elements<S>(g, n < 64 ? (int)n : 64);
     const int64_t nvec = (n - head) / K;
     const u32x4 *body = (const u32x4 *)(g + head);
-    const int64_t i0 = (int64_t)tile * (kThreads * kUnroll) + threadIdx.x;
-    u32x4 w[kUnroll];
+    const int64_t i0 = tile * kTile + threadIdx.x;
+    u32x4 w[kScaleUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++)
-        if (i0 + u * kThreads < nvec) w[u] = body[i0 + u * kThreads];
+    for (int u = 0; u < kScaleUnroll; u++)
+        if (i0 + u * kScaleThreads < nvec) w[u] = __builtin_nontemporal_load(body + i0 + u * kScaleThreads);
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-        const int64_t i = i0 + u * kThreads;
+    for (int u = 0; u < kScaleUnroll; u++) {
+        const int64_t i = i0 + u * kScaleThreads;
         if (i >= nvec) break;
         float x[K];
         E::unpack(w[u], x);
 #pragma unroll
         for (int k = 0; k < K; k++) x[k] = x[k] * f;
-        typename Elem<D>::Bits *to = o + head + i * K;
-        if (Elem<D>::kVec == K) {
-            *(typename Elem<D>::Vec *)to = Elem<D>::pack(x);
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; k += 4) store4<D>(to + k, 4, x + k);
-        }
+        store_past_cache<D, K>(o + head + i * K, x);
     }
     if (tile == 0) {
         const int64_t tail_lo = head + nvec * K, edge = head + (n - tail_lo);
@@ -185,14 +198,19 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(Batch batch, const
     }
 }
 
-int64_t tile_of(int32_t type) { return type == kFp32 ? tile_elements<Single>() : tile_elements<Half>(); }
 uintptr_t size_of(int32_t type) { return type == kFp32 ? 4 : 2; }
 bool known(int32_t type) { return type == kFp32 || type == kFp16 || type == kBf16; }
-int64_t tiles_of(const bmt_clip_tensor &t) { return t.n <= 0 ? 0 : (t.n + tile_of(t.src_type) - 1) / tile_of(t.src_type); }
+// Tiles of `vectors` 16-byte vectors.
+int64_t tiles_of(const bmt_clip_tensor &t, int64_t vectors) {
+    const int64_t tile = vectors * 16 / (int64_t)size_of(t.src_type);
+    return t.n <= 0 ? 0 : (t.n + tile - 1) / tile;
+}
+constexpr int64_t kNormTile = (int64_t)kThreads * kUnroll, kScaleTile = (int64_t)kScaleThreads * kScaleUnroll;
 
-// Calls launch(batch, tiles) for batches of the tensors with these types.
+// Calls launch(batch, tiles) for batches of the tensors with these types (dst_type < 0: any), in order or backwards.
 template <typename F>
-hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, F launch) {
+hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, int64_t vectors, bool backwards,
+                      F launch) {
     Batch b;
     int held = 0;
     int64_t tiles = 0;
@@ -203,10 +221,10 @@ hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src
         held = 0, tiles = 0;
         return hipGetLastError();
     };
-    for (int32_t k = 0; k < count; k++) {
-        const bmt_clip_tensor &t = tensors[k];
+    for (int32_t j = 0; j < count; j++) {
+        const bmt_clip_tensor &t = tensors[backwards ? count - 1 - j : j];
         if (t.n <= 0 || t.src_type != src_type || (dst_type >= 0 && t.dst_type != dst_type)) continue;
-        const int64_t more = tiles_of(t);
+        const int64_t more = tiles_of(t, vectors);
         if (held == kBatch || tiles + more > 0x7FFFFFFF) {
             const hipError_t e = flush();
             if (e != hipSuccess) return e;
@@ -227,7 +245,7 @@ const char *check_table(int32_t count, const bmt_clip_tensor *tensors, bool with
         if (!t.src || (with_dst && !t.dst)) return "null pointer";
         if ((uintptr_t)t.src % size_of(t.src_type) || (with_dst && (uintptr_t)t.dst % size_of(t.dst_type)))
             return "tensor is not aligned to its elements";
-        if (tiles_of(t) > 0x3FFFFFFF) return "tensor too large for one launch";
+        if (tiles_of(t, kScaleTile) > 0x3FFFFFFF) return "tensor too large for one launch";
     }
     return nullptr;
 }
@@ -266,7 +284,7 @@ const char *check_overlap(int32_t count, const bmt_clip_tensor *tensors) {
 template <typename S>
 hipError_t norm_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t type, bool max, double *partials, int64_t *used,
                        hipStream_t s) {
-    return in_batches(count, tensors, type, -1, [&](const Batch &b, uint32_t tiles) {
+    return in_batches(count, tensors, type, -1, kNormTile, false, [&](const Batch &b, uint32_t tiles) {
         if (max) hipLaunchKernelGGL((grad_norm_kernel<S, true>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
         else hipLaunchKernelGGL((grad_norm_kernel<S, false>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
         *used += tiles;
@@ -276,8 +294,8 @@ hipError_t norm_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t ty
 template <typename S, typename D>
 hipError_t scale_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, const float *coef,
                         int32_t round_coef, hipStream_t s) {
-    return in_batches(count, tensors, src_type, dst_type, [&](const Batch &b, uint32_t tiles) {
-        hipLaunchKernelGGL((grad_scale_kernel<S, D>), dim3(tiles), dim3(kThreads), 0, s, b, coef, round_coef);
+    return in_batches(count, tensors, src_type, dst_type, kScaleTile, true, [&](const Batch &b, uint32_t tiles) {
+        hipLaunchKernelGGL((grad_scale_kernel<S, D>), dim3(tiles), dim3(kScaleThreads), 0, s, b, coef, round_coef);
     });
 }
 template <typename S>
@@ -294,7 +312,7 @@ hipError_t scale_from(int32_t count, const bmt_clip_tensor *tensors, int32_t src
 extern "C" int64_t grad_norm_workspace_doubles(int32_t count, const bmt_clip_tensor *tensors) {
     int64_t tiles = 1;
     if (tensors)
-        for (int32_t k = 0; k < count; k++) tiles += bmt::tiles_of(tensors[k]);
+        for (int32_t k = 0; k < count; k++) tiles += bmt::tiles_of(tensors[k], bmt::kNormTile);
     return tiles;
 }
 
@@ -335,8 +353,8 @@ extern "C" int grad_scale_multi_launcher(int32_t count, const bmt_clip_tensor *t
         return refuse(who, "out of host memory");
     }
     hipStream_t s = (hipStream_t)stream;
-    hipError_t e = scale_from<Single>(count, tensors, kFp32, (const float *)coef, round_coef, s);
+    hipError_t e = scale_from<BFloat16>(count, tensors, kBf16, (const float *)coef, round_coef, s);     // backwards here too
     if (e == hipSuccess) e = scale_from<Half>(count, tensors, kFp16, (const float *)coef, round_coef, s);
-    if (e == hipSuccess) e = scale_from<BFloat16>(count, tensors, kBf16, (const float *)coef, round_coef, s);
+    if (e == hipSuccess) e = scale_from<Single>(count, tensors, kFp32, (const float *)coef, round_coef, s);
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }

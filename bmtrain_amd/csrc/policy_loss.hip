@@ -7,22 +7,24 @@
 // R is the masked mean over all tokens, the mean over the sequences that have tokens of their own masked means, or the
 // masked sum.  Back, with w the token's weight in R:
 //     dl = w ( [not clipped] (-A r) + beta (1 - e^q) ),      dE = -alpha w
-// Which side of a clip a token falls is decided on d in 64 bits against the logarithm of the border, so it does not
-// depend on the rounding of e^d; e^x - 1 - x is a power series near 0, where the difference would leave no digits.
+// Which side of a clip a token falls is decided on the exact d against the logarithm of the border in 64 bits, so it does
+// not depend on the rounding of e^d; e^x - 1 - x is a power series for |x| < 1, where the difference would leave few
+// digits, and e^x comes from the same series.
 // Values under an unset mask are read but never used: whatever stands there leaves no trace.
 //
-// A unit is a row's part of up to 4,096 tokens; 8, 64 or 256 lanes work on one, four tokens to a lane at a time.  The
-// loss pass writes the six sums of a unit (or, where rows are not split, of a workgroup) and the token's unweighted
-// derivative; one workgroup adds the sums in a fixed order; the backward pass multiplies by weight and upstream.  All
-// sums are held in 64 bits.  Bound by HBM for large batches (fp32 with a reference: 13 B read and 4 written per token
-// forward, 4 read and 4 written back), by launches for small ones.
+// A unit is a row's part of 1,024 to 16,384 tokens, fewer in large batches; 8 to 256 lanes work on one, four tokens to a
+// lane at a time.  The loss pass writes the six sums of a unit (or, where rows are not split, of a workgroup) and the
+// token's unweighted derivative; one workgroup adds the sums in a fixed order; the backward pass multiplies by weight and
+// upstream.  Four neighbouring tokens are added in fp32, everything above in 64 bits.  All of a quad's loads are asked for
+// before the first value is used; values that few tokens need (|x| >= 1, ties at a border) are computed behind a branch
+// of the whole wave.  Bound by HBM and the latency of its loads for large batches (1,024 x 8,192 fp32 with reference and
+// entropy: 176 MB in 40 us, 4.4 TB/s; 107 registers leave four waves to a SIMD, and fewer spill), by launches for small.
 #include "bmt_vec.h"
 #include "../../include/bmt_hip.h"
 
 namespace bmt {
 
 constexpr int kSums = 6;             // policy, kl, entropy, clipped, old_kl, tokens (or sequences) counted
-constexpr int kUnitTokens = 4096;
 constexpr int kLossThreads = 256;
 constexpr int kFinishThreads = 1024;
 constexpr int64_t kMaxWorkgroups = 2048;
@@ -35,107 +37,162 @@ struct PolicyIn {
     const uint8_t *mask;                             // null: every token counts
     int64_t logprob_row, old_row, ref_row, entropy_row, advantage_row, mask_row;   // elements between rows
     int32_t advantage_col;                           // 0: one advantage for a whole row; 1: one for each token
-    int32_t rows, time, chunks, reduction;
+    int32_t rows, time, chunks, unit, lanes, reduction;
     double high, low, far;                           // log(1 + hi), log(1 - lo), log(c); far = inf: no dual clip
     float ratio_high, ratio_low, ratio_far, kl_coef;
 };
 
-// e^x - 1 - x
-__device__ __forceinline__ float exp_minus_linear(float x) {
-    if (fabsf(x) < 0.5f) {           // x^2 (1/2 + x/6 + ... + x^7/9!): the first term left out is below 2^-29 of the sum
-        float s = 1.f / 362880.f;
-        s = __builtin_fmaf(s, x, 1.f / 40320.f);
-        s = __builtin_fmaf(s, x, 1.f / 5040.f);
-        s = __builtin_fmaf(s, x, 1.f / 720.f);
-        s = __builtin_fmaf(s, x, 1.f / 120.f);
-        s = __builtin_fmaf(s, x, 1.f / 24.f);
-        s = __builtin_fmaf(s, x, 1.f / 6.f);
-        s = __builtin_fmaf(s, x, 0.5f);
-        return x * x * s;
-    }
-    return expm1f(x) - x;
+// e^x - 1 - x for |x| < 1: x^2 (1/2 + x/6 + ... + x^9/11!), what is left out is below 2^-27 of the sum.
+__device__ __forceinline__ float exp_tail_series(float x) {
+    float s = 1.f / 39916800.f;
+    s = __builtin_fmaf(s, x, 1.f / 3628800.f);
+    s = __builtin_fmaf(s, x, 1.f / 362880.f);
+    s = __builtin_fmaf(s, x, 1.f / 40320.f);
+    s = __builtin_fmaf(s, x, 1.f / 5040.f);
+    s = __builtin_fmaf(s, x, 1.f / 720.f);
+    s = __builtin_fmaf(s, x, 1.f / 120.f);
+    s = __builtin_fmaf(s, x, 1.f / 24.f);
+    s = __builtin_fmaf(s, x, 1.f / 6.f);
+    s = __builtin_fmaf(s, x, 0.5f);
+    return x * x * s;
 }
 
-template <typename T, int LANES>
-__global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, int64_t units, float *__restrict__ saved,
+template <typename T>
+struct Tokens {                      // four tokens as they are in memory
+    Raw4<T> logprob, old, ref, entropy;
+    Raw4<Single> advantage;
+    uint32_t mask;
+};
+
+// The six sums of every thread in v[0..5], over the workgroup: all[0..5] of the slots, valid behind the last barrier.
+__device__ __forceinline__ void workgroup_sums(double *v, double (*slots)[8], double *all) {
+    v[6] = v[7] = 0;
+    const double s = wave_sum8(v);
+    if (threadIdx.x % 8 == 0) slots[threadIdx.x / kWave][threadIdx.x % kWave / 8] = s;
+    __syncthreads();
+    if (threadIdx.x < kSums) {
+        double t = 0;
+        for (int w = 0; w < (int)blockDim.x / kWave; w++) t += slots[w][threadIdx.x];
+        all[threadIdx.x] = t;
+    }
+    __syncthreads();
+}
+
+// kWhole: the workgroup's lanes work on one unit; kGroups: groups of in.lanes lanes of a wave do; kTiny: the same for rows of
+// up to three tokens.
+enum Form { kWhole, kGroups, kTiny };
+template <typename T, Form FORM>
+__global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, uint32_t units, float *__restrict__ saved,
                                                                    float *__restrict__ weights, double *__restrict__ sums) {
     typedef typename Elem<T>::Bits Bits;
-    constexpr int GROUPS = kLossThreads / LANES, WAVES = kLossThreads / kWave;
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    constexpr bool WHOLE = FORM == kWhole;
+    const int lanes = WHOLE ? kLossThreads : in.lanes, groups = kLossThreads / lanes;
+    const int lane = threadIdx.x % lanes, group = WHOLE ? 0 : threadIdx.x / lanes, step = lanes * 4;
     const bool split = in.chunks > 1;
-    __shared__ double slots[WAVES][kSums];
-    double total[kSums] = {0, 0, 0, 0, 0, 0};
-    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < units; first += (int64_t)gridDim.x * GROUPS) {
-        const int64_t unit = first + group;
-        double acc[kSums] = {0, 0, 0, 0, 0, 0};
+    __shared__ double slots[kLossThreads / kWave][8], all[8];
+    double total[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const float high = (float)in.high, low = (float)in.low, far = (float)in.far;
+    for (uint32_t first = blockIdx.x * groups; first < units; first += gridDim.x * groups) {
+        const uint32_t unit = first + group;
         const bool there = unit < units;
-        const int32_t row = there ? (int32_t)(unit / in.chunks) : 0;
-        const int begin = there ? (int)(unit - (int64_t)row * in.chunks) * kUnitTokens : in.time;
-        const int end = there ? (in.time - begin < kUnitTokens ? in.time : begin + kUnitTokens) : 0;
+        const int64_t row = there ? unit / (uint32_t)in.chunks : 0;
+        const int begin = there ? (int)(unit - (uint32_t)row * (uint32_t)in.chunks) * in.unit : 0;
+        const int end = there ? (in.time - begin < in.unit ? in.time : begin + in.unit) : 0;
         const Bits *lp = (const Bits *)in.logprob + row * in.logprob_row;
         const Bits *op = (const Bits *)in.old + row * in.old_row;
-        const Bits *fp = (const Bits *)in.ref + (in.ref ? row * in.ref_row : 0);
-        const Bits *ep = (const Bits *)in.entropy + (in.entropy ? row * in.entropy_row : 0);
+        const Bits *fp = in.ref ? (const Bits *)in.ref + row * in.ref_row : lp;      // absent: q = 0, nothing comes of it
+        const Bits *ep = (const Bits *)in.entropy + row * in.entropy_row;
         const uint8_t *mp = in.mask ? in.mask + row * in.mask_row : nullptr;
         const float *ap = in.advantage + row * in.advantage_row;
-        for (int i = begin + lane * 4; i < end; i += LANES * 4) {
-            const int count = end - i;
-            float l[4], o[4], f[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0}, a[4], g[4];
-            const uint32_t m = mask4(mp ? mp + i : nullptr, count);
-            load4<T>(lp + i, count, l);
-            load4<T>(op + i, count, o);
-            if (in.ref) load4<T>(fp + i, count, f);
-            if (in.entropy) load4<T>(ep + i, count, e);
-            if (in.advantage_col) load4<Single>((const uint32_t *)ap + i, count, a);
-            else a[0] = a[1] = a[2] = a[3] = ap[0];
+        const float row_advantage = there && !in.advantage_col ? ap[0] : 0.f;
+        double acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int i = begin + lane * 4; i < end; i += step) {
+            // The last quad of a row that has fewer than four tokens left starts further in front and leaves out what it
+            // shares with its neighbour, so that all loads are whole (a row of one to three tokens has no room for that).
+            const int at = FORM == kTiny || i + 4 <= end ? i : end - 4, skip = i - at;
+            Tokens<T> now;
+            if (FORM == kTiny) {
+                now.mask = load_mask4(mp ? mp + at : nullptr, end - at);
+                now.logprob.load_some(lp + at, end - at);
+                now.old.load_some(op + at, end - at);
+                now.ref.load_some(fp + at, end - at);
+                if (in.entropy) now.entropy.load_some(ep + at, end - at);
+                if (in.advantage_col) now.advantage.load_some((const uint32_t *)ap + at, end - at);
+            } else {
+                now.mask = mp ? *(const u32_any1 *)(mp + at) : 0x01010101u;
+                now.logprob.load(lp + at);
+                now.old.load(op + at);
+                now.ref.load(fp + at);
+                if (in.entropy) now.entropy.load(ep + at);
+                if (in.advantage_col) now.advantage.load((const uint32_t *)ap + at);
+                now.mask &= 0xFFFFFFFFu << (8 * skip);
+            }
+            float sum[5] = {0, 0, 0, 0, 0};               // of these four tokens
+            float g[4], most = 0.f;
+            bool tie = false;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const double wide = (double)l[k] - (double)o[k];
-                const float d = (float)wide, r = expf(d), A = a[k];
-                float policy = -r * A, slope = -r * A;
-                bool clipped = false;
-                if (A > 0.f) {
-                    if (wide > in.high) clipped = true, policy = -in.ratio_high * A;
-                } else if (A < 0.f) {
-                    if (wide < in.low) clipped = true, policy = -in.ratio_low * A;
-                    else if (wide > in.far) clipped = true, policy = -in.ratio_far * A;
+                const float l = now.logprob.get(k), d = l - now.old.get(k);
+                const float A = in.advantage_col ? now.advantage.get(k) : row_advantage;
+                most = fmaxf(most, fmaxf(fabsf(d), fabsf(now.ref.get(k) - l)));
+                tie |= d == high || d == low || d == far || !(d == d) || !(A == A);
+            }
+            const bool plain = !__any(!(most < 1.f) || tie);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float l = now.logprob.get(k), o = now.old.get(k), d = l - o, q = now.ref.get(k) - l;
+                const float A = in.advantage_col ? now.advantage.get(k) : row_advantage;
+                float old_kl = exp_tail_series(d), rm1 = d + old_kl;       // e^d - 1 - d, e^d - 1
+                float kl = exp_tail_series(q), qm1 = q + kl;
+                // rounding keeps the order, so the rounded d against a rounded border is the answer unless they are equal
+                bool over = A > 0.f ? d > high : A < 0.f && d > far, under = A < 0.f && d < low;
+                if (!plain) {
+                    const double wide = (double)l - (double)o;
+                    over = A > 0.f ? wide > in.high : A < 0.f && wide > in.far;
+                    under = A < 0.f && wide < in.low;
+                    if (!(fabsf(d) < 1.f)) rm1 = expf(d) - 1.f, old_kl = rm1 - d;
+                    if (!(fabsf(q) < 1.f)) qm1 = expf(q) - 1.f, kl = qm1 - q;
                 }
-                if (clipped) slope = 0.f;
-                float kl = 0.f;
-                if (in.ref) {
-                    const float q = (float)((double)f[k] - (double)l[k]);
-                    kl = exp_minus_linear(q);
-                    slope = __builtin_fmaf(-in.kl_coef, expm1f(q), slope);
-                }
-                const bool on = m >> k & 1u;
+                const float r = over ? (A > 0.f ? in.ratio_high : in.ratio_far) : under ? in.ratio_low : 1.f + rm1;
+                const float policy = -r * A;
+                const float slope = __builtin_fmaf(-in.kl_coef, qm1, over || under ? 0.f : policy);
+                const bool on = mask_set(now.mask, k);
                 g[k] = on ? slope : 0.f;
-                if (on) {
-                    acc[0] += (double)policy;
-                    acc[1] += (double)kl;
-                    acc[2] += (double)e[k];
-                    acc[3] += clipped ? 1.0 : 0.0;
-                    acc[4] += (double)exp_minus_linear(d);
-                    acc[5] += 1.0;
+                sum[0] += on ? policy : 0.f;
+                sum[1] += on ? kl : 0.f;
+                sum[2] += on && in.entropy ? now.entropy.get(k) : 0.f;
+                sum[3] += on && (over || under) ? 1.f : 0.f;
+                sum[4] += on ? old_kl : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 5; k++) acc[k] += (double)sum[k];
+            acc[5] += (double)mask_count(now.mask);
+            if (saved) {
+                uint32_t *to = (uint32_t *)saved + row * in.time + at;
+                if (FORM == kTiny) {
+                    store4<Single>(to, end - at, g);
+                } else if (skip == 0) {
+                    store4<Single>(to, 4, g);
+                } else {
+#pragma unroll
+                    for (int k = 1; k < 4; k++)
+                        if (k >= skip) to[k] = Elem<Single>::put(g[k]);
                 }
             }
-            if (saved) store4<Single>((uint32_t *)saved + (int64_t)row * in.time + i, count, g);
         }
         if (!split && in.reduction == kSequence) {        // the row is this group's: its own mean
+            if (WHOLE) {
+                workgroup_sums(acc, slots, all);
 #pragma unroll
-            for (int k = 0; k < kSums; k++) acc[k] = lanes_sum(acc[k], LANES < kWave ? LANES : kWave);
-            if (LANES > kWave) {
-                __syncthreads();
-                if (threadIdx.x % kWave == 0)
-                    for (int k = 0; k < kSums; k++) slots[threadIdx.x / kWave][k] = acc[k];
-                __syncthreads();
-                for (int k = 0; k < kSums; k++) {
-                    acc[k] = 0;
-                    for (int w = 0; w < WAVES; w++) acc[k] += slots[w][k];
-                }
+                for (int k = 0; k < kSums; k++) acc[k] = all[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSums; k++) acc[k] = lanes_sum(acc[k], lanes);
             }
             const double weight = acc[5] > 0 ? 1.0 / acc[5] : 0.0;
             if (lane == 0 && there) {
                 weights[1 + row] = (float)weight;
+#pragma unroll
                 for (int k = 0; k < 5; k++) total[k] += acc[k] * weight;
                 total[5] += acc[5] > 0 ? 1.0 : 0.0;
             }
@@ -143,19 +200,10 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
 #pragma unroll
             for (int k = 0; k < kSums; k++) total[k] += acc[k];
         }
-        if (split) break;                                 // one unit to a workgroup: its sums are joined by row
     }
-#pragma unroll
-    for (int k = 0; k < kSums; k++) total[k] = lanes_sum(total[k], kWave);
     __syncthreads();
-    if (threadIdx.x % kWave == 0)
-        for (int k = 0; k < kSums; k++) slots[threadIdx.x / kWave][k] = total[k];
-    __syncthreads();
-    if (threadIdx.x < kSums) {
-        double v = 0;
-        for (int w = 0; w < WAVES; w++) v += slots[w][threadIdx.x];
-        sums[(int64_t)blockIdx.x * kSums + threadIdx.x] = v;
-    }
+    workgroup_sums(total, slots, all);
+    if (threadIdx.x < kSums) sums[(int64_t)blockIdx.x * kSums + threadIdx.x] = all[threadIdx.x];
 }
 
 // Adds the sums of all workgroups.  by_row: `parts` = rows x chunks, and every row's mean is formed first.
@@ -166,7 +214,7 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
                                                                        float entropy_coef, float *__restrict__ weights,
                                                                        float *__restrict__ loss, float *__restrict__ stats) {
     const bool by_row = reduction == kSequence && chunks > 1;
-    double acc[kSums] = {0, 0, 0, 0, 0, 0};
+    double acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (by_row) {
         const int64_t rows = parts / chunks;
         for (int64_t r = threadIdx.x; r < rows; r += kFinishThreads) {
@@ -182,19 +230,8 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
         for (int64_t p = threadIdx.x; p < parts; p += kFinishThreads)
             for (int k = 0; k < kSums; k++) acc[k] += sums[p * kSums + k];
     }
-    __shared__ double slots[kFinishThreads / kWave][kSums];
-#pragma unroll
-    for (int k = 0; k < kSums; k++) acc[k] = lanes_sum(acc[k], kWave);
-    if (threadIdx.x % kWave == 0)
-        for (int k = 0; k < kSums; k++) slots[threadIdx.x / kWave][k] = acc[k];
-    __syncthreads();
-    __shared__ double all[kSums];
-    if (threadIdx.x < kSums) {
-        double v = 0;
-        for (int w = 0; w < kFinishThreads / kWave; w++) v += slots[w][threadIdx.x];
-        all[threadIdx.x] = v;
-    }
-    __syncthreads();
+    __shared__ double slots[kFinishThreads / kWave][8], all[8];
+    workgroup_sums(acc, slots, all);
     if (threadIdx.x == 0) {
         const double share = reduction == kSum ? 1.0 : all[5] > 0 ? 1.0 / all[5] : 0.0;     // nothing counts: loss 0
         for (int k = 0; k < 5; k++) all[k] *= share;
@@ -224,25 +261,32 @@ __global__ __launch_bounds__(kLossThreads) void policy_backward_kernel(
         store4<T>(grad + at, count, g);
     }
     if (grad_entropy) {
-        const uint32_t m = mask4(mask ? mask + row * mask_row + i : nullptr, count);
+        const uint32_t m = load_mask4(mask ? mask + row * mask_row + i : nullptr, count);
         float g[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) g[k] = m >> k & 1u ? -entropy_coef * scale : 0.f;
+        for (int k = 0; k < 4; k++) g[k] = mask_set(m, k) ? -entropy_coef * scale : 0.f;
         store4<T>(grad_entropy + at, count, g);
     }
 }
 
 struct Shape {
     int lanes;
-    int32_t chunks;
+    int32_t unit, chunks;
     int64_t units, grid;
 };
-// Lanes to a unit: a row of up to 32 tokens is eight lanes' (four tokens each), one of up to 1,024 a wave's, anything
-// longer a workgroup's.  Rows that are split get a workgroup for every part.
+// A row of up to 256 tokens is that of 8 to 64 lanes, four tokens each; up to 1,024 it is a workgroup's while there are few
+// rows, where it is the latency that counts, and a wave's when there are many.  Longer rows are split into parts of a
+// workgroup each, the shortest from 1,024 to 16,384 tokens that give at most 1,024 parts: a workgroup's start and its
+// sums cost as much as some 2,000 tokens (8.4 M tokens fp32 with reference and entropy: 45 us in parts of 8,192 tokens,
+// 48 of 4,096, 51 of 2,048, 66 of 1,024; both launches).
 static Shape shape_of(int64_t rows, int64_t time) {
     Shape s;
-    s.chunks = (int32_t)((time + kUnitTokens - 1) / kUnitTokens);
-    s.lanes = time <= 32 ? 8 : time <= 1024 ? 64 : 256;
+    s.unit = 1024;
+    while (s.unit < 16384 && rows * ((time + s.unit - 1) / s.unit) > 1024) s.unit *= 2;
+    s.chunks = (int32_t)((time + s.unit - 1) / s.unit);
+    s.lanes = 8;
+    while (s.lanes < 64 && s.lanes * 4 < time) s.lanes *= 2;
+    if (time > 1024 || (time > 256 && rows < 4096)) s.lanes = kLossThreads;
     s.units = rows * s.chunks;
     const int64_t groups = kLossThreads / s.lanes;
     s.grid = (s.units + groups - 1) / groups;
@@ -252,20 +296,20 @@ static Shape shape_of(int64_t rows, int64_t time) {
 
 template <typename T>
 static void loss_launch(const PolicyIn &in, const Shape &s, float *saved, float *weights, double *sums, hipStream_t stream) {
-    if (s.lanes == 8)
-        hipLaunchKernelGGL((policy_loss_kernel<T, 8>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, s.units, saved,
-                           weights, sums);
-    else if (s.lanes == 64)
-        hipLaunchKernelGGL((policy_loss_kernel<T, 64>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, s.units, saved,
-                           weights, sums);
+    if (s.lanes == kLossThreads)
+        hipLaunchKernelGGL((policy_loss_kernel<T, kWhole>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
+                           saved, weights, sums);
+    else if (in.time >= 4)
+        hipLaunchKernelGGL((policy_loss_kernel<T, kGroups>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
+                           saved, weights, sums);
     else
-        hipLaunchKernelGGL((policy_loss_kernel<T, 256>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, s.units, saved,
-                           weights, sums);
+        hipLaunchKernelGGL((policy_loss_kernel<T, kTiny>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
+                           saved, weights, sums);
 }
 
 static bool fits(int64_t rows, int64_t time) {
     return rows <= 0x7FFFFFFF && time <= 0x3FFFFFFF && (rows * ((time + 3) / 4)) / kLossThreads < 0x7FFFFFFF &&
-           rows * ((time + kUnitTokens - 1) / kUnitTokens) < 0x7FFFFFFF;
+           rows * ((time + 1023) / 1024) < 0x7FFFFFFF;
 }
 
 }  // namespace bmt
@@ -293,7 +337,7 @@ extern "C" int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t 
     if ((uintptr_t)workspace % 8 || ((uintptr_t)loss | (uintptr_t)stats | (uintptr_t)saved | (uintptr_t)weights) % 4)
         return refuse(who, "misaligned output");
     hipStream_t s = (hipStream_t)stream;
-    Shape shape = {64, 1, 0, 0};
+    Shape shape = {64, 1024, 1, 0, 0};
     if (rows > 0 && time > 0) {
         if (!fits(rows, time)) return refuse(who, "too many tokens for one launch");
         if (!logprob || !old_logprob || !advantage) return refuse(who, "null pointer");
@@ -308,7 +352,7 @@ extern "C" int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t 
         in.advantage = (const float *)advantage, in.mask = (const uint8_t *)mask;
         in.logprob_row = logprob_row, in.old_row = old_row, in.ref_row = ref_row, in.entropy_row = entropy_row;
         in.advantage_row = advantage_row, in.mask_row = mask_row, in.advantage_col = advantage_col;
-        in.rows = (int32_t)rows, in.time = (int32_t)time, in.chunks = shape.chunks, in.reduction = reduction;
+        in.rows = (int32_t)rows, in.time = (int32_t)time, in.chunks = shape.chunks, in.unit = shape.unit, in.lanes = shape.lanes, in.reduction = reduction;
         in.high = log1p(clip_high), in.low = log1p(-clip_low);          // clip_low = 1: log 0 = -inf, never below it
         in.far = dual_clip != 0 ? log(dual_clip) : (double)INFINITY;
         in.ratio_high = (float)(1 + clip_high), in.ratio_low = (float)(1 - clip_low), in.ratio_far = (float)dual_clip;

@@ -11,7 +11,7 @@
 // Back: dl[i, t] = +-m (dloss/dh) / pairs (/ n_i), the sign that of the row.
 // h is a small difference of large sums, so the sums and everything per pair are held in 64 bits.
 //
-// A unit is a row's part of up to 4,096 tokens (8, 64 or 256 lanes); one workgroup turns the units' sums into pairs.
+// A unit is a row's part of up to 1,024 tokens (4,096 in large batches; 8, 64 or 256 lanes); one workgroup turns the units' sums into pairs.
 // Bound by HBM for large batches (fp32: 9 B read per token forward, 1 read and 4 written back), by launches for small.
 #include "bmt_vec.h"
 #include "../../include/bmt_hip.h"
@@ -19,7 +19,6 @@
 namespace bmt {
 namespace {
 
-constexpr int kUnitTokens = 4096;
 constexpr int kThreads = 256;
 constexpr int kPairThreads = 1024;
 
@@ -32,7 +31,7 @@ struct RowSum {
 
 template <typename T, int LANES>
 __global__ __launch_bounds__(kThreads) void preference_sum_kernel(
-    int64_t units, int32_t chunks, int32_t time, const typename Elem<T>::Bits *__restrict__ logprob, int64_t logprob_row,
+    int64_t units, int32_t chunks, int32_t part, int32_t time, const typename Elem<T>::Bits *__restrict__ logprob, int64_t logprob_row,
     const typename Elem<T>::Bits *__restrict__ ref, int64_t ref_row, const uint8_t *__restrict__ mask, int64_t mask_row,
     RowSum *__restrict__ sums) {
     typedef typename Elem<T>::Bits Bits;
@@ -43,21 +42,31 @@ __global__ __launch_bounds__(kThreads) void preference_sum_kernel(
     int tokens = 0;
     if (unit < units) {
         const int64_t row = unit / chunks;
-        const int begin = (int)(unit - row * chunks) * kUnitTokens;
-        const int end = time - begin < kUnitTokens ? time : begin + kUnitTokens;
+        const int begin = (int)(unit - row * chunks) * part;
+        const int end = time - begin < part ? time : begin + part;
         const Bits *lp = logprob + row * logprob_row;
         const Bits *fp = ref ? ref + row * ref_row : nullptr;
         const uint8_t *mp = mask ? mask + row * mask_row : nullptr;
         for (int i = begin + lane * 4; i < end; i += LANES * 4) {
-            const int count = end - i;
-            float l[4], f[4] = {0, 0, 0, 0};
-            const uint32_t m = mask4(mp ? mp + i : nullptr, count);
-            load4<T>(lp + i, count, l);
-            if (fp) load4<T>(fp + i, count, f);
+            // the last quad of a row starts further in front and leaves out what it shares with its neighbour, so that
+            // all loads are whole; a row of one to three tokens has no room for that
+            const int at = time < 4 || i + 4 <= end ? i : end - 4;
+            uint32_t m;
+            Raw4<T> l, f;
+            if (time >= 4) {
+                m = mp ? *(const u32_any1 *)(mp + at) : 0x01010101u;
+                l.load(lp + at);
+                if (fp) f.load(fp + at);
+                m &= 0xFFFFFFFFu << (8 * (i - at));
+            } else {
+                m = load_mask4(mp ? mp + at : nullptr, end - at);
+                l.load_some(lp + at, end - at);
+                if (fp) f.load_some(fp + at, end - at);
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (m >> k & 1u) sum += (double)l[k] - (double)f[k];
-            tokens += __popc(m);
+                if (mask_set(m, k)) sum += (double)l.get(k) - (fp ? (double)f.get(k) : 0.0);
+            tokens += mask_count(m);
         }
     }
     sum = lanes_sum(sum, LANES < kWave ? LANES : kWave);
@@ -140,37 +149,39 @@ __global__ __launch_bounds__(kThreads) void preference_backward_kernel(int32_t t
     if (q >= quads) return;
     const int64_t row = q / quads_per_row;
     const int i = (int)(q - row * quads_per_row) * 4, count = time - i;
-    const uint32_t m = mask4(mask ? mask + row * mask_row + i : nullptr, count);
+    const uint32_t m = load_mask4(mask ? mask + row * mask_row + i : nullptr, count);
     const float v = slope[1 + row] * (upstream[0] * slope[0]);
     float g[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) g[k] = m >> k & 1u ? v : 0.f;
+    for (int k = 0; k < 4; k++) g[k] = mask_set(m, k) ? v : 0.f;
     store4<T>(grad + row * (int64_t)time + i, count, g);
 }
 
-int64_t chunks_of(int64_t time) { return time <= 0 ? 1 : (time + kUnitTokens - 1) / kUnitTokens; }
+// Tokens of a unit: one step of a workgroup's lanes up to 4,096 units, four beyond.
+int64_t part_of(int64_t pairs, int64_t time) { return 2 * pairs * ((time + 1023) / 1024) <= 4096 ? 1024 : 4096; }
+int64_t chunks_of(int64_t pairs, int64_t time) { return time <= 0 ? 1 : (time + part_of(pairs, time) - 1) / part_of(pairs, time); }
 
 bool fits(int64_t pairs, int64_t time) {
     return pairs <= 0x3FFFFFFF && time <= 0x3FFFFFFF && 2 * pairs * ((time + 3) / 4) / kThreads < 0x7FFFFFFF &&
-           2 * pairs * chunks_of(time) < 0x7FFFFFFF;
+           2 * pairs * ((time + 1023) / 1024) < 0x7FFFFFFF;
 }
 
 template <typename T, int LANES>
 void sum_launch(int64_t rows, int64_t time, const void *logprob, int64_t logprob_row, const void *ref, int64_t ref_row,
                 const void *mask, int64_t mask_row, RowSum *sums, hipStream_t s) {
-    const int64_t chunks = chunks_of(time), units = rows * chunks, groups = kThreads / LANES;
+    const int64_t chunks = chunks_of(rows / 2, time), units = rows * chunks, groups = kThreads / LANES;
     typedef typename Elem<T>::Bits Bits;
     hipLaunchKernelGGL((preference_sum_kernel<T, LANES>), dim3((unsigned)((units + groups - 1) / groups)), dim3(kThreads), 0, s, units,
-                       (int32_t)chunks, (int32_t)time, (const Bits *)logprob, logprob_row, (const Bits *)ref, ref_row,
+                       (int32_t)chunks, (int32_t)part_of(rows / 2, time), (int32_t)time, (const Bits *)logprob, logprob_row, (const Bits *)ref, ref_row,
                        (const uint8_t *)mask, mask_row, sums);
 }
-// A row of up to 32 tokens is eight lanes' (four tokens each), one of up to 1,024 a wave's, a part of a longer one a
-// workgroup's.
+// A row of up to 32 tokens is eight lanes' (four tokens each), one of up to 256 a wave's, of up to 1,024 a workgroup's
+// while there are few rows and a wave's when there are many, and a part of a longer one a workgroup's.
 template <typename T>
 void sum_pick(int64_t rows, int64_t time, const void *logprob, int64_t logprob_row, const void *ref, int64_t ref_row,
               const void *mask, int64_t mask_row, RowSum *sums, hipStream_t s) {
     if (time <= 32) sum_launch<T, 8>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
-    else if (time <= 1024) sum_launch<T, 64>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
+    else if (time <= 256 || (time <= 1024 && rows >= 4096)) sum_launch<T, 64>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
     else sum_launch<T, 256>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
 }
 
@@ -179,7 +190,7 @@ void sum_pick(int64_t rows, int64_t time, const void *logprob, int64_t logprob_r
 
 extern "C" int64_t preference_loss_workspace_doubles(int64_t pairs, int64_t time) {
     if (pairs <= 0 || !bmt::fits(pairs, time)) return 1;
-    return 2 * pairs * bmt::chunks_of(time) * 2;
+    return 2 * pairs * bmt::chunks_of(pairs, time) * 2;
 }
 
 extern "C" int preference_loss_forward_launcher(int64_t pairs, int64_t time, int32_t type, const void *logprob, int64_t logprob_row,
@@ -208,7 +219,7 @@ extern "C" int preference_loss_forward_launcher(int64_t pairs, int64_t time, int
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return fail((int)e, who, e);
     }
-    hipLaunchKernelGGL(preference_pair_kernel, dim3(1), dim3(kPairThreads), 0, s, pairs, (int32_t)chunks_of(time), sums, kind, average,
+    hipLaunchKernelGGL(preference_pair_kernel, dim3(1), dim3(kPairThreads), 0, s, pairs, (int32_t)chunks_of(pairs, time), sums, kind, average,
                        beta, label_smoothing, (float *)loss, (float *)chosen, (float *)rejected, (float *)slope);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail((int)e, who, e);

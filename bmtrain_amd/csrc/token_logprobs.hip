@@ -88,10 +88,8 @@ __device__ __forceinline__ void online_add(Online &a, const float *x, float c) {
     a.m = top;
 }
 
-constexpr int kForwardUnroll = 4;
-
-// ROW: threads to a row (64: the workgroup's four waves take a row each).
-template <typename T, int ROW, bool ENTROPY>
+// ROW: threads to a row (64: the workgroup's four waves take a row each); UNROLL: vectors of a lane in flight.
+template <typename T, int ROW, int UNROLL, bool ENTROPY>
 __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     LogitRows in, Targets target, float inv_t, float *__restrict__ logprob, float *__restrict__ entropy,
     RowStats *__restrict__ stats) {
@@ -120,19 +118,27 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     Online a = {-__FLT_MAX__, 0.f, 0.f};
     constexpr int K = E::kVec;
     int i = lane;
-    for (; i + (kForwardUnroll - 1) * ROW < nvec; i += kForwardUnroll * ROW) {
-        u32x4 w[kForwardUnroll];
-        float v[kForwardUnroll * K];
+    for (; i + (UNROLL - 1) * ROW < nvec; i += UNROLL * ROW) {
+        u32x4 w[UNROLL];
+        float v[UNROLL * K];
 #pragma unroll
-        for (int u = 0; u < kForwardUnroll; u++) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
+        for (int u = 0; u < UNROLL; u++) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
 #pragma unroll
-        for (int u = 0; u < kForwardUnroll; u++) E::unpack(w[u], v + u * K);
-        online_add<ENTROPY, kForwardUnroll * K>(a, v, c);
+        for (int u = 0; u < UNROLL; u++) E::unpack(w[u], v + u * K);
+        online_add<ENTROPY, UNROLL * K>(a, v, c);
     }
-    for (; i < nvec; i += ROW) {
-        float v[K];
-        E::unpack(__builtin_nontemporal_load(body + i), v);
-        online_add<ENTROPY, K>(a, v, c);
+    {       // fewer than UNROLL vectors are left to this lane: all are requested before the first is used
+        u32x4 w[UNROLL - 1];
+#pragma unroll
+        for (int u = 0; u < UNROLL - 1; u++)
+            if (i + u * ROW < nvec) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
+#pragma unroll
+        for (int u = 0; u < UNROLL - 1; u++) {
+            if (i + u * ROW >= nvec) break;
+            float v[K];
+            E::unpack(w[u], v);
+            online_add<ENTROPY, K>(a, v, c);
+        }
     }
     const int tail_lo = head + nvec * K, edge = head + (n - tail_lo);      // fewer than 2 * kVec elements
     if (lane < edge) {
@@ -160,16 +166,19 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     }
 }
 
-constexpr int kBackwardUnroll = 4;
+// Workgroups of consecutive tiles on one XCD: 32 against one, two vectors to a lane in both: 664 / 697 us on 8,192 x 128,256
+// bf16 with entropies, 326 / 334 on 16,384 x 32,000 fp16 (6.4 TB/s); 16 to 128 measure alike, 4 and 512 are slower.
+constexpr uint32_t kBackwardRun = 32;
 
-template <typename T, int ROW, bool ENTROPY>
+// A tile is UNROLL vectors of ROW lanes; tiles are numbered through the rows.
+template <typename T, int ROW, int UNROLL, bool ENTROPY>
 __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
     LogitRows in, Targets target, float inv_t, const RowStats *__restrict__ stats, const float *__restrict__ grad_logprob,
     const float *__restrict__ grad_entropy, typename Elem<T>::Bits *__restrict__ grad, int32_t tiles) {
     typedef Elem<T> E;
     constexpr int PER = 256 / ROW, K = E::kVec;
     const int lane = threadIdx.x % ROW;
-    const uint32_t unit = blockIdx.x * PER + threadIdx.x / ROW;
+    const uint32_t unit = xcd_run<kBackwardRun>(blockIdx.x, gridDim.x) * PER + threadIdx.x / ROW;
     const int32_t r = (int32_t)(unit / (uint32_t)tiles), tile = (int32_t)(unit - (uint32_t)r * (uint32_t)tiles);
     if (PER > 1 && r >= in.rows) return;
     const int64_t t = target.at(r);
@@ -193,15 +202,15 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
         const float p = __builtin_amdgcn_exp2f((z - st.log_sum) * kLog2e);
         return p * (ENTROPY ? __builtin_fmaf(b, fmaxf(z, kFar) + shift, a) : a);
     };
-    const int i0 = tile * (ROW * kBackwardUnroll) + lane;
-    u32x4 w[kBackwardUnroll];
+    const int i0 = tile * (ROW * UNROLL) + lane;
+    u32x4 w[UNROLL];
     if (live) {
 #pragma unroll
-        for (int u = 0; u < kBackwardUnroll; u++)
+        for (int u = 0; u < UNROLL; u++)
             if (i0 + u * ROW < nvec) w[u] = __builtin_nontemporal_load(body + i0 + u * ROW);
     }
 #pragma unroll
-    for (int u = 0; u < kBackwardUnroll; u++) {
+    for (int u = 0; u < UNROLL; u++) {
         const int i = i0 + u * ROW;
         if (i >= nvec) break;
         u32x4 packed = {0u, 0u, 0u, 0u};
@@ -248,47 +257,58 @@ static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void
     return nullptr;
 }
 
-template <typename T, int ROW, bool ENTROPY>
+template <typename T, int ROW, int UNROLL, bool ENTROPY>
 static void forward_launch(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                            hipStream_t stream) {
     constexpr int PER = ROW < 256 ? 256 / ROW : 1;
     const unsigned grid = (unsigned)((in.rows + (int64_t)PER - 1) / PER);
-    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, ENTROPY>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
+    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
                        logprob, entropy, stats);
 }
+template <typename T, int ROW, int UNROLL>
+static void forward_rows(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+                         hipStream_t stream) {
+    if (entropy) forward_launch<T, ROW, UNROLL, true>(in, t, inv_t, logprob, entropy, stats, stream);
+    else forward_launch<T, ROW, UNROLL, false>(in, t, inv_t, logprob, entropy, stats, stream);
+}
+// Threads to a row by its vectors: eight or more to a lane.  Measured (us, 256 / 512 / 1,024 threads): 16,384 x 32,000 fp16
+// 156 / 147 / 190, 8,192 x 128,256 bf16 with entropies 314 / 309 / 304, 20,000 x 5,000 fp16 46 / 63 / 103, one row of
+// 128,256 17.7 / 12.0 / 11.8.  Vectors of a lane in flight, 2 / 3 / 4 / 8: 311 / 300 / 306 / 387 on 8,192 x 128,256 and
+// 45 / 41 / 51 / 67 on 30,000 x 4,000.
 template <typename T>
 static void forward_pick(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                          hipStream_t stream) {
-    if (in.n <= kWaveRow) {
-        if (entropy) forward_launch<T, 64, true>(in, t, inv_t, logprob, entropy, stats, stream);
-        else forward_launch<T, 64, false>(in, t, inv_t, logprob, entropy, stats, stream);
-    } else {
-        if (entropy) forward_launch<T, 256, true>(in, t, inv_t, logprob, entropy, stats, stream);
-        else forward_launch<T, 256, false>(in, t, inv_t, logprob, entropy, stats, stream);
-    }
+    const int32_t vectors = in.n / Elem<T>::kVec;
+    if (in.n <= kWaveRow) forward_rows<T, 64, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    else if (vectors < 2048) forward_rows<T, 256, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    else if (vectors < 12288) forward_rows<T, 512, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    else forward_rows<T, 1024, 3>(in, t, inv_t, logprob, entropy, stats, stream);
 }
 
-template <typename T, int ROW>
+template <typename T, int ROW, int UNROLL>
 static const char *backward_launch(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
                                    const float *ge, void *grad, hipStream_t stream) {
-    const int64_t per_tile = (int64_t)ROW * kBackwardUnroll * Elem<T>::kVec;
+    const int64_t per_tile = (int64_t)ROW * UNROLL * Elem<T>::kVec;
     const int64_t tiles = (in.n + per_tile - 1) / per_tile, per = 256 / ROW;
     const int64_t grid = (in.rows * tiles + per - 1) / per;
     if (in.rows * tiles > 0x7FFFFFFF) return "too many elements for one launch";
     typedef typename Elem<T>::Bits Bits;
     if (ge)
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, true>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
                            stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     else
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, false>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, false>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
                            stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     return nullptr;
 }
 template <typename T>
 static const char *backward_pick(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
                                  const float *ge, void *grad, hipStream_t stream) {
-    return in.n <= kWaveRow ? backward_launch<T, 64>(in, t, inv_t, stats, gl, ge, grad, stream)
-                            : backward_launch<T, 256>(in, t, inv_t, stats, gl, ge, grad, stream);
+    if (in.n <= kWaveRow) return backward_launch<T, 64, 4>(in, t, inv_t, stats, gl, ge, grad, stream);
+    // two vectors to a lane where a row has four such tiles or more (664 us against 683 with four on 8,192 x 128,256 bf16);
+    // a shorter row leaves much of its last tile idle and needs more in flight (20,000 x 5,000 fp16: 83 us with two, 67)
+    if (in.n > 4 * 512 * Elem<T>::kVec) return backward_launch<T, 256, 2>(in, t, inv_t, stats, gl, ge, grad, stream);
+    return backward_launch<T, 256, 4>(in, t, inv_t, stats, gl, ge, grad, stream);
 }
 
 }  // namespace bmt

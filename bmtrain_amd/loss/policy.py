@@ -32,33 +32,30 @@ class OpPolicyLoss(torch.autograd.Function):
     """Loss and statistics in two launches, both gradients in one."""
 
     @staticmethod
-    def forward(ctx, logprob, entropy, old_logprob, advantages, mask, ref_logprob, clip_low, clip_high, dual_clip, kl_coef,
-                entropy_coef, reduction):
-        rows, time = logprob.shape
-        device = logprob.device
+    def forward(ctx, logprob, entropy, old_logprob, advantages, mask, ref_logprob, clips, kl_coef, entropy_coef, reduction):
         with F.on_device_of(logprob):
+            shape, device = logprob.shape, logprob.device
+            offsets = F.policy_loss_scratch(*shape, reduction == 1, ctx.needs_input_grad[0])
             loss = torch.empty((), device=device, dtype=torch.float)
             stats = torch.empty(5, device=device, dtype=torch.float)
-            weights = torch.empty(1 + rows if reduction == 1 else 1, device=device, dtype=torch.float)
-            workspace = torch.empty(C.policy_loss_workspace_doubles(rows, time), device=device, dtype=torch.double)
-            saved = torch.empty((rows, time), device=device, dtype=torch.float) if ctx.needs_input_grad[0] else None
-            F.policy_loss_forward(logprob, old_logprob, ref_logprob, entropy, advantages, mask, clip_low, clip_high, dual_clip,
-                                  kl_coef, entropy_coef, reduction, saved, weights, workspace, loss, stats)
-        ctx.args = (reduction, entropy_coef, logprob.shape, logprob.dtype)
+            scratch = torch.empty(offsets[0], device=device, dtype=torch.float)
+            F.policy_loss_forward(logprob, old_logprob, ref_logprob, entropy, advantages, mask, *clips, kl_coef, entropy_coef,
+                                  reduction, scratch, offsets, loss, stats)
+        ctx.args = (reduction, offsets, entropy_coef, shape, logprob.dtype)
         ctx.mark_non_differentiable(stats)
-        ctx.save_for_backward(saved, weights, mask)
+        ctx.save_for_backward(scratch, mask)
         return loss, stats
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, _):
-        saved, weights, mask = ctx.saved_tensors
-        reduction, entropy_coef, shape, dtype = ctx.args
-        with F.on_device_of(weights):
-            grads = [torch.empty(shape, device=weights.device, dtype=dtype) if needed else None
-                     for needed in ctx.needs_input_grad[:2]]
-            F.policy_loss_backward(reduction, saved, weights, upstream, mask, entropy_coef, *grads)
-        return (*grads,) + (None,) * 10
+        scratch, mask = ctx.saved_tensors
+        reduction, offsets, entropy_coef, shape, dtype = ctx.args
+        with F.on_device_of(scratch):
+            grad_logprob, grad_entropy = [torch.empty(shape, device=scratch.device, dtype=dtype) if needed else None
+                                          for needed in ctx.needs_input_grad[:2]]
+            F.policy_loss_backward(reduction, scratch, offsets, upstream, mask, entropy_coef, grad_logprob, grad_entropy)
+        return grad_logprob, grad_entropy, None, None, None, None, None, None, None, None
 
 
 class PolicyLoss(torch.nn.Module):
@@ -111,9 +108,13 @@ class PolicyLoss(torch.nn.Module):
         if advantages.dim() == 2 and advantages.size(0) and (advantages.shape != logprob.shape or advantages.stride(1) == 0):
             assert advantages.size(1) == 1 or advantages.shape == logprob.shape, "advantages must be one to a sequence or one to a token"
             advantages = advantages[:, 0]              # one to a sequence: [sequences, 1], or an expanded view
-        advantages = advantages.detach().float()
-        if advantages.dim() == 2:
-            advantages = _tokens_adjacent(advantages)
+        if advantages.dtype != torch.float32:
+            advantages = advantages.float()
+        if advantages.dim() == 1:
+            advantages = advantages.detach() if advantages.requires_grad else advantages
+        else:
+            advantages = constant(advantages)
         return OpPolicyLoss.apply(_tokens_adjacent(logprob), _tokens_adjacent(entropy), constant(old_logprob), advantages,
-                                  as_mask(mask), constant(ref_logprob), self.clip_low, self.clip_high,
-                                  self.dual_clip or 0.0, self.kl_coef, self.entropy_coef, _REDUCTIONS[self.reduction])
+                                  as_mask(mask), constant(ref_logprob),
+                                  (self.clip_low, self.clip_high, self.dual_clip or 0.0), self.kl_coef, self.entropy_coef,
+                                  _REDUCTIONS[self.reduction])

@@ -17,29 +17,29 @@ class OpPreferenceLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logprob, ref_logprob, mask, kind, average, beta, label_smoothing):
-        pairs, time = logprob.size(0) // 2, logprob.size(1)
-        device = logprob.device
         with F.on_device_of(logprob):
+            shape, device = logprob.shape, logprob.device
+            pairs = shape[0] // 2
+            offsets = F.preference_loss_scratch(pairs, shape[1])
             loss = torch.empty((), device=device, dtype=torch.float)
             chosen = torch.empty(pairs, device=device, dtype=torch.float)
             rejected = torch.empty(pairs, device=device, dtype=torch.float)
-            slope = torch.empty(1 + 2 * pairs, device=device, dtype=torch.float)
-            workspace = torch.empty(C.preference_loss_workspace_doubles(pairs, time), device=device, dtype=torch.double)
-            F.preference_loss_forward(logprob, ref_logprob, mask, kind, average, beta, label_smoothing, workspace, loss, chosen,
-                                      rejected, slope)
-        ctx.args = (logprob.shape, logprob.dtype)
+            scratch = torch.empty(offsets[0], device=device, dtype=torch.float)
+            F.preference_loss_forward(logprob, ref_logprob, mask, kind, average, beta, label_smoothing, scratch, offsets, loss,
+                                      chosen, rejected)
+        ctx.args = (offsets, shape, logprob.dtype)
         ctx.mark_non_differentiable(chosen, rejected)
-        ctx.save_for_backward(slope, mask)
+        ctx.save_for_backward(scratch, mask)
         return loss, chosen, rejected
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, *_):
-        slope, mask = ctx.saved_tensors
-        shape, dtype = ctx.args
-        with F.on_device_of(slope):
-            grad = torch.empty(shape, device=slope.device, dtype=dtype)
-            F.preference_loss_backward(slope, upstream, mask, grad)
+        scratch, mask = ctx.saved_tensors
+        offsets, shape, dtype = ctx.args
+        with F.on_device_of(scratch):
+            grad = torch.empty(shape, device=scratch.device, dtype=dtype)
+            F.preference_loss_backward(scratch, offsets, upstream, mask, grad)
         return grad, None, None, None, None, None, None
 
 

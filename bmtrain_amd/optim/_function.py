@@ -208,23 +208,37 @@ def adam_multi(tensors, beta1: float, beta2: float, eps: float, lr: float, scale
 
 
 _TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_Tensor = torch.Tensor
 
 
-def clip_rows(grads, outs=None):
-    """Entries (source, destination, n, type codes) of ``C.clip_table`` for dense GPU tensors of fp32, fp16 or bf16 on one
-    device; ``outs`` (default: the gradients themselves) have their gradients' shapes and strides."""
-    rows = []
-    device = grads[0].device if grads else None
-    for g, o in zip(grads, grads if outs is None else outs):
-        if g.dtype not in _TYPE_CODES or o.dtype not in _TYPE_CODES:
-            raise ValueError(f"gradients must be fp32, fp16 or bf16, not {g.dtype} to {o.dtype}")
-        assert g.is_cuda and g.device == device and o.device == device, "gradients must be on one cuda device"
-        if not g.is_contiguous() or (o is not g and not o.is_contiguous()):
-            assert is_dense(g), "gradients must not have gaps nor elements that share memory"
-            assert o.stride() == g.stride(), "outputs must have their gradients' strides"
-        assert o.shape == g.shape, "outputs must have their gradients' shapes"
-        rows.append((g.data_ptr(), o.data_ptr(), g.numel(), _TYPE_CODES[g.dtype], _TYPE_CODES[o.dtype]))
-    return rows
+def _codes(tensors):
+    codes = [_TYPE_CODES.get(t.dtype) for t in tensors]
+    if None in codes:
+        raise ValueError(f"gradients must be fp32, fp16 or bf16, not {tensors[codes.index(None)].dtype}")
+    return codes
+
+
+def clip_table(grads, outs=None):
+    """``C.clip_table`` of dense GPU tensors of fp32, fp16 or bf16 on one device; ``outs`` (default: the gradients
+    themselves) have their gradients' shapes and strides.  Every property is read once for the whole list: with many
+    small gradients this is what a call costs."""
+    codes = _codes(grads)
+    sources = list(map(_Tensor.data_ptr, grads))
+    devices = set(map(_Tensor.get_device, grads))
+    dense = all(map(_Tensor.is_contiguous, grads))
+    if outs is None or outs is grads:
+        out_codes, destinations = codes, sources
+        assert dense or all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
+    else:
+        out_codes = _codes(outs)
+        destinations = list(map(_Tensor.data_ptr, outs))
+        devices.update(map(_Tensor.get_device, outs))
+        assert [g.shape for g in grads] == [o.shape for o in outs], "outputs must have their gradients' shapes"
+        if not (dense and all(map(_Tensor.is_contiguous, outs))):
+            assert all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
+            assert [g.stride() for g in grads] == [o.stride() for o in outs], "outputs must have their gradients' strides"
+    assert len(devices) == 1 and -1 not in devices, "gradients must be on one cuda device"
+    return C.clip_table(sources, destinations, list(map(_Tensor.numel, grads)), codes, out_codes)
 
 
 def is_dense(t: torch.Tensor) -> bool:
@@ -237,19 +251,21 @@ def is_dense(t: torch.Tensor) -> bool:
     return True
 
 
-def grad_norm_multi(rows, use_max: bool, max_norm: float, eps: float, scale: float, out: torch.Tensor) -> None:
+def grad_norm_multi(table, use_max: bool, max_norm: float, eps: float, scale: float, out: torch.Tensor) -> None:
     """``out[0] = n / scale`` and the clipping factor ``out[1] = max_norm * scale / (n + eps)`` for n the L2 norm (or the
-    largest magnitude) over the gradients of ``rows`` (``clip_rows``); ``out`` is two floats."""
+    largest magnitude) over the gradients of ``table`` (``clip_table``); ``out`` is two floats."""
     assert out.is_cuda and out.dtype == torch.float32 and out.numel() == 2 and out.is_contiguous()
-    table = C.clip_table(rows)
-    workspace = torch.empty(C.grad_norm_workspace_doubles(len(rows), table), dtype=torch.float64, device=out.device)
-    C.grad_norm_multi_launcher(len(rows), table, int(use_max), max_norm, eps, scale, workspace.data_ptr(), out.data_ptr(),
-                               _current_stream())
+    address, words = table.buffer_info()
+    device = out.get_device()
+    workspace = torch.empty(C.grad_norm_workspace_doubles(words // 4, address), dtype=torch.float64, device=out.device)
+    C.grad_norm_multi_launcher(words // 4, address, int(use_max), max_norm, eps, scale, workspace.data_ptr(), out.data_ptr(),
+                               torch._C._cuda_getCurrentRawStream(device))
 
 
-def grad_scale_multi(rows, coef: torch.Tensor, round_coef: bool = False) -> None:
-    """Every destination of ``rows`` = its source times ``coef`` (one float on the GPU) if that is below one, else the
+def grad_scale_multi(table, coef: torch.Tensor, round_coef: bool = False) -> None:
+    """Every destination of ``table`` = its source times ``coef`` (one float on the GPU) if that is below one, else the
     source itself; ``round_coef``: times the factor rounded to the source's type."""
     assert coef.is_cuda and coef.dtype == torch.float32 and coef.numel() == 1, "coef must be one float on cuda"
-    if rows:
-        C.grad_scale_multi_launcher(len(rows), C.clip_table(rows), coef.data_ptr(), int(round_coef), _current_stream())
+    address, words = table.buffer_info()
+    C.grad_scale_multi_launcher(words // 4, address, coef.data_ptr(), int(round_coef),
+                                torch._C._cuda_getCurrentRawStream(coef.get_device()))

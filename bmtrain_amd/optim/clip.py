@@ -6,7 +6,13 @@ from typing import Optional, Sequence
 
 import torch
 
+from ..loss._function import on_device_of
 from . import _function as F
+
+
+def _is_none(t):
+    return t is None
+
 
 
 @torch.no_grad()
@@ -39,7 +45,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(outs)} outputs")
-    if any(g is None for g in grads):
+    if any(map(_is_none, grads)):
         outs = [o for g, o in zip(grads, outs) if g is not None]
         grads = [g for g in grads if g is not None]
     if not (max_norm >= 0 and eps >= 0 and scale > 0 and math.isfinite(scale)):
@@ -49,9 +55,9 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         raise ValueError(f"norm_type must be 2 or inf, not {norm_type}")
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda" if torch.cuda.is_available() else "cpu")
-    rows = F.clip_rows(grads, outs)
-    with torch.cuda.device(grads[0].device):
+    table = F.clip_table(grads, outs)
+    with on_device_of(grads[0]):
         result = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-        F.grad_norm_multi(rows, use_max, float(max_norm), float(eps), float(scale), result)
-        F.grad_scale_multi(rows, result[1])
+        F.grad_norm_multi(table, use_max, float(max_norm), float(eps), float(scale), result)
+        F.grad_scale_multi(table, result[1])
     return result[0]

@@ -220,5 +220,5 @@ def test_rounded_factor():
     coef = torch.tensor(0.123456, device="cuda")
     grads = grads_of([1001, 999, 1003], (torch.float32, torch.bfloat16, torch.float16), 6)
     want = [(g.float() * coef.to(g.dtype).float()).to(g.dtype) for g in grads]
-    OF.grad_scale_multi(OF.clip_rows(grads), coef, round_coef=True)
+    OF.grad_scale_multi(OF.clip_table(grads), coef, round_coef=True)
     assert all(torch.equal(a, b) for a, b in zip(grads, want))

@@ -110,7 +110,7 @@ def test_policy_entry():
     C.policy_loss_backward_launcher(0, 8, 0, 0, 0, 0, 0, 0, 0, 0.0, 0x1000, 0, 0)
     with pytest.raises(RuntimeError, match="null"):
         C.policy_loss_backward_launcher(2, 8, 0, 0, 0, 0x2000, 0x3000, 0, 0, 0.0, 0x1000, 0, 0)
-    assert C.policy_loss_workspace_doubles(0, 5) == 1 and C.policy_loss_workspace_doubles(3, 9000) == 3 * 3 * 6
+    assert C.policy_loss_workspace_doubles(0, 5) == 1 and C.policy_loss_workspace_doubles(3, 9000) == 3 * 9 * 6 and C.policy_loss_workspace_doubles(1024, 8192) == 1024 * 6
 
 
 def preference(pairs=2, time=8, code=0, logprob=0x1000, kind=0, beta=0.1, smoothing=0.0, workspace=0x2000, loss=0x3000, chosen=0x4000,
@@ -131,7 +131,8 @@ def test_preference_entry():
 
 def test_clip_entries():
     def scale(rows, coef=0x100000):
-        C.grad_scale_multi_launcher(len(rows), C.clip_table(rows), coef, 0, 0)
+        table = C.clip_table(*[list(column) for column in zip(*rows)]) if rows else C.clip_table([], [], [], [], [])
+        C.grad_scale_multi_launcher(len(rows), table.buffer_info()[0], coef, 0, 0)
     scale([])
     scale([(0, 0, 0, 0, 0)])                                                # entries without elements are skipped
     a, b = 0x10000, 0x20000
@@ -143,9 +144,10 @@ def test_clip_entries():
             scale(rows)
     with pytest.raises(RuntimeError, match="null"):
         scale([(a, b, 10, 0, 0)], coef=0)
-    table = C.clip_table([(a, 0, 10, 0, 0)])
+    table = C.clip_table([a], [0], [10], [0], [0])
+    address = table.buffer_info()[0]
     with pytest.raises(RuntimeError, match="scale"):
-        C.grad_norm_multi_launcher(1, table, 0, 1.0, 1e-6, 0.0, 0x1000, 0x2000, 0)
+        C.grad_norm_multi_launcher(1, address, 0, 1.0, 1e-6, 0.0, 0x1000, 0x2000, 0)
     with pytest.raises(RuntimeError, match="null"):
-        C.grad_norm_multi_launcher(1, table, 0, 1.0, 1e-6, 1.0, 0, 0x2000, 0)
-    assert C.grad_norm_workspace_doubles(1, table) == 2 and C.grad_norm_workspace_doubles(0, None) == 1
+        C.grad_norm_multi_launcher(1, address, 0, 1.0, 1e-6, 1.0, 0, 0x2000, 0)
+    assert C.grad_norm_workspace_doubles(1, address) == 2 and C.grad_norm_workspace_doubles(0, 0) == 1
