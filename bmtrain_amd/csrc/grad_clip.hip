@@ -255,23 +255,24 @@ const char *check_table(int32_t count, const bmt_clip_tensor *tensors, bool with
 const char *check_overlap(int32_t count, const bmt_clip_tensor *tensors) {
     struct Span {
         uintptr_t begin, end;
-        int32_t entry;
         bool out;
     };
-    std::vector<Span> spans;
-    spans.reserve(2 * (size_t)count);
+    // inputs and outputs apart: gradients are often allocated in order, as are the places they go to
+    std::vector<Span> spans, outs;
+    spans.reserve(2 * (size_t)count), outs.reserve((size_t)count);
     for (int32_t k = 0; k < count; k++) {
         const bmt_clip_tensor &t = tensors[k];
         if (t.n <= 0) continue;
         const uintptr_t s = (uintptr_t)t.src, d = (uintptr_t)t.dst;
-        if (s == d && t.src_type == t.dst_type) {
-            spans.push_back({d, d + (uintptr_t)t.n * size_of(t.dst_type), k, true});
-        } else {
-            spans.push_back({s, s + (uintptr_t)t.n * size_of(t.src_type), k, false});
-            spans.push_back({d, d + (uintptr_t)t.n * size_of(t.dst_type), k, true});
-        }
+        if (s != d || t.src_type != t.dst_type) spans.push_back({s, s + (uintptr_t)t.n * size_of(t.src_type), false});
+        outs.push_back({d, d + (uintptr_t)t.n * size_of(t.dst_type), true});
     }
-    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+    auto before = [](const Span &a, const Span &b) { return a.begin < b.begin; };
+    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+    if (!std::is_sorted(outs.begin(), outs.end(), before)) std::sort(outs.begin(), outs.end(), before);
+    const size_t inputs = spans.size();
+    spans.insert(spans.end(), outs.begin(), outs.end());
+    std::inplace_merge(spans.begin(), spans.begin() + (std::ptrdiff_t)inputs, spans.end(), before);
     uintptr_t out_end = 0, any_end = 0;                  // how far outputs / anything in front of here reach
     for (const Span &s : spans) {
         if (s.begin < out_end || (s.out && s.begin < any_end)) return "an output shares memory with another tensor of the call";

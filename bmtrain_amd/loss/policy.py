@@ -13,7 +13,7 @@ _REDUCTIONS = {"mean": 0, "sequence": 1, "sum": 2}
 
 def _tokens_adjacent(t):
     """`t` with its last dimension's elements next to each other (a copy where they are not); None stays None."""
-    return t if t is None or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.is_contiguous() or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def constant(t):

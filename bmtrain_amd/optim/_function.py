@@ -212,18 +212,21 @@ _Tensor = torch.Tensor
 
 
 def _codes(tensors):
-    codes = [_TYPE_CODES.get(t.dtype) for t in tensors]
-    if None in codes:
-        raise ValueError(f"gradients must be fp32, fp16 or bf16, not {tensors[codes.index(None)].dtype}")
-    return codes
+    dtypes = [t.dtype for t in tensors]
+    kinds = set(dtypes)
+    for dtype in kinds:
+        if dtype not in _TYPE_CODES:
+            raise ValueError(f"gradients must be fp32, fp16 or bf16, not {dtype}")
+    return [_TYPE_CODES[dtypes[0]]] * len(dtypes) if len(kinds) == 1 else [_TYPE_CODES[dtype] for dtype in dtypes]
 
 
 def clip_table(grads, outs=None):
     """``C.clip_table`` of dense GPU tensors of fp32, fp16 or bf16 on one device; ``outs`` (default: the gradients
-    themselves) have their gradients' shapes and strides.  Every property is read once for the whole list: with many
-    small gradients this is what a call costs."""
+    themselves) have their gradients' numbers of elements, and their strides where a gradient is not contiguous.  Every
+    property is read once for the whole list: with many small gradients this is what a call costs."""
     codes = _codes(grads)
     sources = list(map(_Tensor.data_ptr, grads))
+    counts = list(map(_Tensor.numel, grads))
     devices = set(map(_Tensor.get_device, grads))
     dense = all(map(_Tensor.is_contiguous, grads))
     if outs is None or outs is grads:
@@ -233,12 +236,13 @@ def clip_table(grads, outs=None):
         out_codes = _codes(outs)
         destinations = list(map(_Tensor.data_ptr, outs))
         devices.update(map(_Tensor.get_device, outs))
-        assert [g.shape for g in grads] == [o.shape for o in outs], "outputs must have their gradients' shapes"
+        assert counts == list(map(_Tensor.numel, outs)), "outputs must have their gradients' numbers of elements"
         if not (dense and all(map(_Tensor.is_contiguous, outs))):
             assert all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
-            assert [g.stride() for g in grads] == [o.stride() for o in outs], "outputs must have their gradients' strides"
+            assert all((g.is_contiguous() and o.is_contiguous()) or (g.shape == o.shape and g.stride() == o.stride())
+                       for g, o in zip(grads, outs)), "outputs must have their gradients' strides"
     assert len(devices) == 1 and -1 not in devices, "gradients must be on one cuda device"
-    return C.clip_table(sources, destinations, list(map(_Tensor.numel, grads)), codes, out_codes)
+    return C.clip_table(sources, destinations, counts, codes, out_codes)
 
 
 def is_dense(t: torch.Tensor) -> bool:

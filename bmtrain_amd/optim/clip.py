@@ -31,8 +31,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         max_norm: the largest norm of the unscaled gradients.
         norm_type: 2.0, or ``math.inf`` / ``'inf'`` for the largest magnitude.
         scale: the loss scale the gradients carry; the returned norm is divided by it.
-        out: tensors of the gradients' shapes (and strides, where not contiguous), of any of the three types, that
-            receive the clipped gradients - fp32 accumulators into the 16-bit gradients of an optimizer, say; ``None``
+        out: tensors of as many elements as the gradients (of their shapes and strides, where those are not contiguous),
+            of any of the three types, that receive the clipped gradients - fp32 accumulators into the 16-bit gradients of an optimizer, say; ``None``
             clips in place.  An output may be its own gradient but share memory with nothing else of the call
             (``RuntimeError``; the gradients themselves are not listed twice either when they are clipped in place).
 
@@ -60,4 +60,6 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         result = torch.empty(2, dtype=torch.float32, device=grads[0].device)
         F.grad_norm_multi(table, use_max, float(max_norm), float(eps), float(scale), result)
         F.grad_scale_multi(table, result[1])
+    if not torch.is_inference_mode_enabled():
+        torch.autograd.graph.increment_version(outs)        # autograd is to notice the write, as with any in-place operation
     return result[0]

@@ -10,9 +10,9 @@ from typing import Optional
 import torch
 
 from ..global_var import config
-from ..loss._function import has_inf_nan
+from ..loss._function import has_inf_nan, on_device_of
 from ._base import flat_runs
-from ._function import grad_stats, grad_stats_multi
+from ._function import clip_table, grad_scale_multi, grad_stats, grad_stats_multi
 
 
 def _scanned_grads(param_groups):
@@ -217,18 +217,32 @@ class OptimManager:
 
     @staticmethod
     def _scale_grads(parameters, clip_coef):
-        """`p.grad.mul_(clip_coef)` for every parameter (optim_manager.py:196-199).  Back-to-back gradients
-        are scaled by one launch.  The factor is handed over as a Python number equal to what the tensor form
-        uses on the GPU — the 0-dim fp32 tensor rounded to the gradient's dtype — which takes torch's
-        vectorised scalar kernel: same bits, 3x faster."""
-        as_number = {}
-        for g in flat_runs([p.grad.data for p in parameters if p.grad is not None]):
-            if g.is_cuda and g.dtype in (torch.float16, torch.bfloat16, torch.float32):
-                if g.dtype not in as_number:
-                    as_number[g.dtype] = float(clip_coef.to(g.dtype))
-                g.mul_(as_number[g.dtype])
+        """`p.grad.mul_(clip_coef)` for every parameter if clip_coef < 1 (optim_manager.py:196-199).  Contiguous GPU
+        gradients take one launch per 96 runs of back-to-back ones, which looks at the factor on the GPU: no host read.
+        The factor is rounded to each gradient's type there, as torch does with a 0-dim fp32 factor: same bits."""
+        runs = flat_runs([p.grad.data for p in parameters if p.grad is not None])
+        fused, rest, end = [], [], 0
+        for g in sorted(runs, key=lambda g: g.data_ptr()):
+            # a gradient met twice (or one that overlaps another) is scaled twice: one after the other, below
+            if (torch.is_tensor(clip_coef) and clip_coef.is_cuda and clip_coef.dtype == torch.float32 and g.is_cuda
+                    and g.device == clip_coef.device and g.is_contiguous() and g.numel() and g.data_ptr() >= end
+                    and g.dtype in (torch.float16, torch.bfloat16, torch.float32)):
+                fused.append(g)
+                end = g.data_ptr() + g.numel() * g.element_size()
             else:
-                g.mul_(clip_coef)
+                rest.append(g)
+        if fused:
+            with on_device_of(fused[0]):
+                grad_scale_multi(clip_table(fused), clip_coef, round_coef=True)
+        if rest and clip_coef < 1:
+            as_number = {}                  # on the GPU a Python number takes torch's vectorised scalar kernel: same bits
+            for g in rest:
+                if g.is_cuda and g.dtype in (torch.float16, torch.bfloat16, torch.float32):
+                    if g.dtype not in as_number:
+                        as_number[g.dtype] = float(clip_coef.to(g.dtype))
+                    g.mul_(as_number[g.dtype])
+                else:
+                    g.mul_(clip_coef)
 
     def clip_grad_norm(self, param_groups, max_norm, norm_type=2, eps=1e-6):
         """Clips the (still loss-scaled) gradients to ``max_norm`` in place and returns the
@@ -267,11 +281,10 @@ class OptimManager:
                     acc += g.float().norm(norm_type) ** norm_type
             total_norm = acc[0] ** (1.0 / norm_type)
         clip_coef = float(max_norm * scale) / (total_norm + eps)
-        if clip_coef < 1:
-            if self._can_defer(parameters):
-                self._pending_clip = (clip_coef, with_grad)          # applied by the next step()
-            else:
-                self._scale_grads(with_grad, clip_coef)
+        if not self._can_defer(parameters):
+            self._scale_grads(with_grad, clip_coef)
+        elif clip_coef < 1:
+            self._pending_clip = (clip_coef, with_grad)              # applied by the next step()
         # The pass over the 16-bit gradients also looked for inf / NaN, and the scaling above cannot change that
         # verdict (it multiplies by a finite factor below one, or by zero when the norm itself is infinite);
         # step() reuses it for gradients that nobody has written to since.

@@ -95,6 +95,13 @@ def test_dense_layouts():
         clip_grads([base[:1].expand(4, 70, 5)], 1.0)
     with pytest.raises(AssertionError, match="strides"):
         clip_grads([base.transpose(0, 1)], 1.0, out=[torch.empty(70, 60, 5, device="cuda")])
+    with pytest.raises(AssertionError, match="strides"):
+        clip_grads([base], 1.0, out=[torch.empty(70, 60, 5, device="cuda").transpose(0, 1)])
+    flat = torch.empty(60 * 70 * 5, device="cuda", dtype=torch.bfloat16)               # contiguous: any shape will do
+    clip_grads([base], 0.1, out=[flat])
+    want = torch.empty_like(base, dtype=torch.bfloat16)
+    clip_grads([base], 0.1, out=[want])
+    assert torch.equal(flat, want.flatten())
 
 
 def test_squares_outside_fp32():
@@ -161,7 +168,7 @@ def test_refusals():
     check([g[0], g[0]], 1.0, out=[torch.empty_like(g[0]), torch.empty_like(g[0])])     # read twice, written once each
     with pytest.raises(ValueError, match="float64"):
         clip_grads([g[0].double()], 1.0)
-    with pytest.raises(AssertionError, match="shapes"):
+    with pytest.raises(AssertionError, match="numbers of elements"):
         clip_grads([g[0]], 1.0, out=[g[1]])
     assert float(clip_grads([], 1.0)) == 0.0
     assert float(clip_grads([None, g[1]], 1e9, out=[None, torch.empty_like(g[1])])) > 0
@@ -213,6 +220,24 @@ def test_manager_scales_with_the_same_bits(dtypes):
         norm = manager.clip_grad_norm([{"params": [twice, twice]}], max_norm)
         coef = float(max_norm * 8.0) / (norm * 8.0 + 1e-6)
         assert torch.equal(twice.grad, b.mul_(coef).mul_(coef) if coef < 1 else b)
+
+
+def test_autograd_notices_the_write():
+    x = torch.full((100,), 2.0, device="cuda", requires_grad=True)
+    saved = x.detach().clone()
+    y = (saved * x).sum()                                           # keeps `saved` for its backward pass
+    clip_grads([saved], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_a_larger_grid_than_one_batch_of_every_type():
+    """More tensors than a launch takes, types mixed, outputs of mixed types."""
+    sizes = [(k * 37) % 999 + 1 for k in range(500)]
+    kinds = (torch.float32, torch.bfloat16, torch.float16, torch.float32, torch.bfloat16)
+    grads = grads_of(sizes, kinds, 13)
+    check(grads, 0.2, out=[torch.empty_like(g, dtype=kinds[k % 3]) for k, g in enumerate(grads)])
+    check(grads, 0.2)
 
 
 def test_rounded_factor():
