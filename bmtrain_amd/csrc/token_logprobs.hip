@@ -22,7 +22,8 @@ namespace bmt {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// z behind which e^z is 0 in fp32 (the smallest subnormal is e^-103.3): keeps 0 * -inf out of the entropy's sums
+// exponent behind which a probability is 0 in fp32 (the smallest subnormal is 2^-149): keeps 0 * -inf out of the entropy's
+// sums and gradients
 constexpr float kFar = -1000.f;
 
 struct RowStats {       // what the backward pass needs of a row
@@ -48,6 +49,11 @@ struct Targets {
         return is_64 ? ((const int64_t *)t)[r] : (int64_t)((const int32_t *)t)[r];
     }
 };
+
+template <bool PAST>
+__device__ __forceinline__ u32x4 load_vector(const u32x4 *p) {
+    return PAST ? __builtin_nontemporal_load(p) : *p;
+}
 
 // Running maximum m, s = sum 2^z and w = sum 2^z z with z = (x - m) * c in units of log 2.
 struct Online {
@@ -88,8 +94,9 @@ __device__ __forceinline__ void online_add(Online &a, const float *x, float c) {
     a.m = top;
 }
 
-// ROW: threads to a row (64: the workgroup's four waves take a row each); UNROLL: vectors of a lane in flight.
-template <typename T, int ROW, int UNROLL, bool ENTROPY>
+// ROW: threads to a row (64: the workgroup's four waves take a row each); UNROLL: vectors of a lane in flight; PAST: the
+// logits are read past the caches.
+template <typename T, int ROW, int UNROLL, bool ENTROPY, bool PAST>
 __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     LogitRows in, Targets target, float inv_t, float *__restrict__ logprob, float *__restrict__ entropy,
     RowStats *__restrict__ stats) {
@@ -122,7 +129,7 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
         u32x4 w[UNROLL];
         float v[UNROLL * K];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
+        for (int u = 0; u < UNROLL; u++) w[u] = load_vector<PAST>(body + i + u * ROW);
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) E::unpack(w[u], v + u * K);
         online_add<ENTROPY, UNROLL * K>(a, v, c);
@@ -131,7 +138,7 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
         u32x4 w[UNROLL - 1];
 #pragma unroll
         for (int u = 0; u < UNROLL - 1; u++)
-            if (i + u * ROW < nvec) w[u] = __builtin_nontemporal_load(body + i + u * ROW);
+            if (i + u * ROW < nvec) w[u] = load_vector<PAST>(body + i + u * ROW);
 #pragma unroll
         for (int u = 0; u < UNROLL - 1; u++) {
             if (i + u * ROW >= nvec) break;
@@ -194,13 +201,13 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
     const u32x4 *body = (const u32x4 *)(x + head);
     typename E::Vec *out = (typename E::Vec *)(d + head);
     const RowStats st = live ? stats[r] : RowStats{0.f, 0.f, 0.f, 0.f};
-    const float a = -g * inv_t, b = -h * inv_t;
-    const float shift = st.entropy - st.log_sum;
-
+    // p = 2^y with y = (x - max) * c - log2(sum), log p = y ln 2:  dx = p (a + b y), a = -(g + h H) / T, b = -h ln 2 / T
+    const float c = inv_t * kLog2e, log2_sum = st.log_sum * kLog2e;
+    const float hot = g * inv_t, b = -h * inv_t * kLn2, a = -(g + h * st.entropy) * inv_t;
     auto one = [&](float v) {
-        const float z = (v - st.max) * inv_t;
-        const float p = __builtin_amdgcn_exp2f((z - st.log_sum) * kLog2e);
-        return p * (ENTROPY ? __builtin_fmaf(b, fmaxf(z, kFar) + shift, a) : a);
+        const float y = __builtin_fmaf(v - st.max, c, -log2_sum);
+        const float p = __builtin_amdgcn_exp2f(y);
+        return p * (ENTROPY ? __builtin_fmaf(b, fmaxf(y, kFar), a) : a);
     };
     const int i0 = tile * (ROW * UNROLL) + lane;
     u32x4 w[UNROLL];
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
             if ((uint64_t)at < (uint64_t)K) {
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    if (k == (int)at) v[k] -= a;
+                    if (k == (int)at) v[k] += hot;
             }
             packed = E::pack(v);
         }
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
         float v = 0.f;
         if (live) {
             v = one(E::get(x[j]));
-            if (j == t) v -= a;
+            if (j == t) v += hot;
         }
         d[j] = E::put(v);
     }
@@ -257,19 +264,27 @@ static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void
     return nullptr;
 }
 
-template <typename T, int ROW, int UNROLL, bool ENTROPY>
+template <typename T, int ROW, int UNROLL, bool ENTROPY, bool PAST>
 static void forward_launch(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                            hipStream_t stream) {
     constexpr int PER = ROW < 256 ? 256 / ROW : 1;
     const unsigned grid = (unsigned)((in.rows + (int64_t)PER - 1) / PER);
-    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
+    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY, PAST>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
                        logprob, entropy, stats);
 }
+// Logits of up to this many bytes go through the caches on the way forward: what the 256 MiB of the last level keep of
+// them is there when the backward pass reads them again.  Both passes, through / past the caches: 412 MB of fp32 196 / 203
+// us, 154 MB of bf16 77 / 81; 1.05 GB of fp16 508 / 498, 2.1 GB of bf16 1,021 / 995.
+constexpr int64_t kKeepBytes = (int64_t)512 << 20;
+
 template <typename T, int ROW, int UNROLL>
 static void forward_rows(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                          hipStream_t stream) {
-    if (entropy) forward_launch<T, ROW, UNROLL, true>(in, t, inv_t, logprob, entropy, stats, stream);
-    else forward_launch<T, ROW, UNROLL, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    const bool past = (int64_t)in.rows * in.n * (int64_t)sizeof(typename Elem<T>::Bits) > kKeepBytes;
+    if (entropy && past) forward_launch<T, ROW, UNROLL, true, true>(in, t, inv_t, logprob, entropy, stats, stream);
+    else if (entropy) forward_launch<T, ROW, UNROLL, true, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    else if (past) forward_launch<T, ROW, UNROLL, false, true>(in, t, inv_t, logprob, entropy, stats, stream);
+    else forward_launch<T, ROW, UNROLL, false, false>(in, t, inv_t, logprob, entropy, stats, stream);
 }
 // Threads to a row by its vectors: eight or more to a lane.  Measured (us, 256 / 512 / 1,024 threads): 16,384 x 32,000 fp16
 // 156 / 147 / 190, 8,192 x 128,256 bf16 with entropies 314 / 309 / 304, 20,000 x 5,000 fp16 46 / 63 / 103, one row of
