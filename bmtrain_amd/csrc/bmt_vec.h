@@ -190,6 +190,9 @@ __device__ __forceinline__ V lanes_sum(V v, int lanes) {
     return v;
 }
 
+// Host side: whether a launch of `grid` workgroups of `threads` is within the 2^32 threads that a dispatch can count.
+inline bool launch_fits(int64_t grid, int64_t threads) { return grid * threads < ((int64_t)1 << 32); }
+
 // Host side: refuses a call of C entry `who` because of `why`.
 inline int refuse(const char *who, const char *why) {
     char text[200];

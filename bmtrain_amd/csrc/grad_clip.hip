@@ -209,8 +209,8 @@ constexpr int64_t kNormTile = (int64_t)kThreads * kUnroll, kScaleTile = (int64_t
 
 // Calls launch(batch, tiles) for batches of the tensors with these types (dst_type < 0: any), in order or backwards.
 template <typename F>
-hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, int64_t vectors, bool backwards,
-                      F launch) {
+hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, int64_t vectors, int threads,
+                      bool backwards, F launch) {
     Batch b;
     int held = 0;
     int64_t tiles = 0;
@@ -225,7 +225,7 @@ hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src
         const bmt_clip_tensor &t = tensors[backwards ? count - 1 - j : j];
         if (t.n <= 0 || t.src_type != src_type || (dst_type >= 0 && t.dst_type != dst_type)) continue;
         const int64_t more = tiles_of(t, vectors);
-        if (held == kBatch || tiles + more > 0x7FFFFFFF) {
+        if (held == kBatch || !launch_fits(tiles + more, threads)) {
             const hipError_t e = flush();
             if (e != hipSuccess) return e;
         }
@@ -245,7 +245,7 @@ const char *check_table(int32_t count, const bmt_clip_tensor *tensors, bool with
         if (!t.src || (with_dst && !t.dst)) return "null pointer";
         if ((uintptr_t)t.src % size_of(t.src_type) || (with_dst && (uintptr_t)t.dst % size_of(t.dst_type)))
             return "tensor is not aligned to its elements";
-        if (tiles_of(t, kScaleTile) > 0x3FFFFFFF) return "tensor too large for one launch";
+        if (!launch_fits(tiles_of(t, kScaleTile), kScaleThreads)) return "tensor too large for one launch";
     }
     return nullptr;
 }
@@ -285,7 +285,7 @@ const char *check_overlap(int32_t count, const bmt_clip_tensor *tensors) {
 template <typename S>
 hipError_t norm_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t type, bool max, double *partials, int64_t *used,
                        hipStream_t s) {
-    return in_batches(count, tensors, type, -1, kNormTile, false, [&](const Batch &b, uint32_t tiles) {
+    return in_batches(count, tensors, type, -1, kNormTile, kThreads, false, [&](const Batch &b, uint32_t tiles) {
         if (max) hipLaunchKernelGGL((grad_norm_kernel<S, true>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
         else hipLaunchKernelGGL((grad_norm_kernel<S, false>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
         *used += tiles;
@@ -295,7 +295,7 @@ hipError_t norm_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t ty
 template <typename S, typename D>
 hipError_t scale_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, const float *coef,
                         int32_t round_coef, hipStream_t s) {
-    return in_batches(count, tensors, src_type, dst_type, kScaleTile, true, [&](const Batch &b, uint32_t tiles) {
+    return in_batches(count, tensors, src_type, dst_type, kScaleTile, kScaleThreads, true, [&](const Batch &b, uint32_t tiles) {
         hipLaunchKernelGGL((grad_scale_kernel<S, D>), dim3(tiles), dim3(kScaleThreads), 0, s, b, coef, round_coef);
     });
 }

@@ -308,8 +308,10 @@ static void loss_launch(const PolicyIn &in, const Shape &s, float *saved, float 
 }
 
 static bool fits(int64_t rows, int64_t time) {
-    return rows <= 0x7FFFFFFF && time <= 0x3FFFFFFF && (rows * ((time + 3) / 4)) / kLossThreads < 0x7FFFFFFF &&
-           rows * ((time + 1023) / 1024) < 0x7FFFFFFF;
+    if (rows > 0x7FFFFFFF || time > 0x3FFFFFFF || !launch_fits(rows * ((time + 3) / 4) / kLossThreads + 1, kLossThreads))
+        return false;
+    const Shape s = shape_of(rows, time);
+    return s.units < 0x7FFFFFFF && launch_fits(s.grid, kLossThreads);
 }
 
 }  // namespace bmt

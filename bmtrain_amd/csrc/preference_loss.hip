@@ -161,9 +161,14 @@ __global__ __launch_bounds__(kThreads) void preference_backward_kernel(int32_t t
 int64_t part_of(int64_t pairs, int64_t time) { return 2 * pairs * ((time + 1023) / 1024) <= 4096 ? 1024 : 4096; }
 int64_t chunks_of(int64_t pairs, int64_t time) { return time <= 0 ? 1 : (time + part_of(pairs, time) - 1) / part_of(pairs, time); }
 
+// Lanes to a row of up to 1,024 tokens, or to a part of a longer one: eight lanes for up to 32 tokens (four each), a wave
+// for up to 256; up to 1,024 a workgroup while there are few rows, where it is the latency that counts, and a wave when
+// there are many; a workgroup for a part.
+int lanes_of(int64_t rows, int64_t time) { return time <= 32 ? 8 : time <= 256 || (time <= 1024 && rows >= 4096) ? 64 : kThreads; }
+
 bool fits(int64_t pairs, int64_t time) {
-    return pairs <= 0x3FFFFFFF && time <= 0x3FFFFFFF && 2 * pairs * ((time + 3) / 4) / kThreads < 0x7FFFFFFF &&
-           2 * pairs * ((time + 1023) / 1024) < 0x7FFFFFFF;
+    return pairs <= 0x3FFFFFFF && time <= 0x3FFFFFFF && launch_fits(2 * pairs * ((time + 3) / 4) / kThreads + 1, kThreads) &&
+           launch_fits(2 * pairs * chunks_of(pairs, time) + kThreads, lanes_of(2 * pairs, time));
 }
 
 template <typename T, int LANES>
@@ -175,13 +180,12 @@ void sum_launch(int64_t rows, int64_t time, const void *logprob, int64_t logprob
                        (int32_t)chunks, (int32_t)part_of(rows / 2, time), (int32_t)time, (const Bits *)logprob, logprob_row, (const Bits *)ref, ref_row,
                        (const uint8_t *)mask, mask_row, sums);
 }
-// A row of up to 32 tokens is eight lanes' (four tokens each), one of up to 256 a wave's, of up to 1,024 a workgroup's
-// while there are few rows and a wave's when there are many, and a part of a longer one a workgroup's.
 template <typename T>
 void sum_pick(int64_t rows, int64_t time, const void *logprob, int64_t logprob_row, const void *ref, int64_t ref_row,
               const void *mask, int64_t mask_row, RowSum *sums, hipStream_t s) {
-    if (time <= 32) sum_launch<T, 8>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
-    else if (time <= 256 || (time <= 1024 && rows >= 4096)) sum_launch<T, 64>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
+    const int lanes = lanes_of(rows, time);
+    if (lanes == 8) sum_launch<T, 8>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
+    else if (lanes == 64) sum_launch<T, 64>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
     else sum_launch<T, 256>(rows, time, logprob, logprob_row, ref, ref_row, mask, mask_row, sums, s);
 }
 

@@ -259,18 +259,20 @@ static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void
     if ((uintptr_t)x % (type == kFp32 ? 4 : 2)) return "logits are not aligned to their elements";
     if (target_bits != 32 && target_bits != 64) return "targets have 32 or 64 bits";
     if ((uintptr_t)target % (uintptr_t)(target_bits / 8)) return "targets are not aligned to their elements";
-    if (!(temperature > 0.f) || !(1.f / temperature <= __FLT_MAX__) || !(temperature <= __FLT_MAX__))
+    if (!(temperature > 0.f) || !(kLog2e / temperature <= __FLT_MAX__) || !(temperature <= __FLT_MAX__))
         return "temperature must be positive and finite";
     return nullptr;
 }
 
 template <typename T, int ROW, int UNROLL, bool ENTROPY, bool PAST>
-static void forward_launch(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+static const char *forward_launch(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                            hipStream_t stream) {
     constexpr int PER = ROW < 256 ? 256 / ROW : 1;
     const unsigned grid = (unsigned)((in.rows + (int64_t)PER - 1) / PER);
+    if (!launch_fits(grid, ROW < 256 ? 256 : ROW)) return "too many rows for one launch";
     hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY, PAST>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
                        logprob, entropy, stats);
+    return nullptr;
 }
 // Logits of up to this many bytes go through the caches on the way forward: what the 256 MiB of the last level keep of
 // them is there when the backward pass reads them again.  Both passes, through / past the caches: 412 MB of fp32 196 / 203
@@ -278,26 +280,26 @@ static void forward_launch(const LogitRows &in, const Targets &t, float inv_t, f
 constexpr int64_t kKeepBytes = (int64_t)512 << 20;
 
 template <typename T, int ROW, int UNROLL>
-static void forward_rows(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+static const char *forward_rows(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                          hipStream_t stream) {
     const bool past = (int64_t)in.rows * in.n * (int64_t)sizeof(typename Elem<T>::Bits) > kKeepBytes;
-    if (entropy && past) forward_launch<T, ROW, UNROLL, true, true>(in, t, inv_t, logprob, entropy, stats, stream);
-    else if (entropy) forward_launch<T, ROW, UNROLL, true, false>(in, t, inv_t, logprob, entropy, stats, stream);
-    else if (past) forward_launch<T, ROW, UNROLL, false, true>(in, t, inv_t, logprob, entropy, stats, stream);
-    else forward_launch<T, ROW, UNROLL, false, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (entropy && past) return forward_launch<T, ROW, UNROLL, true, true>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (entropy) return forward_launch<T, ROW, UNROLL, true, false>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (past) return forward_launch<T, ROW, UNROLL, false, true>(in, t, inv_t, logprob, entropy, stats, stream);
+    return forward_launch<T, ROW, UNROLL, false, false>(in, t, inv_t, logprob, entropy, stats, stream);
 }
 // Threads to a row by its vectors: eight or more to a lane.  Measured (us, 256 / 512 / 1,024 threads): 16,384 x 32,000 fp16
 // 156 / 147 / 190, 8,192 x 128,256 bf16 with entropies 314 / 309 / 304, 20,000 x 5,000 fp16 46 / 63 / 103, one row of
 // 128,256 17.7 / 12.0 / 11.8.  Vectors of a lane in flight, 2 / 3 / 4 / 8: 311 / 300 / 306 / 387 on 8,192 x 128,256 and
 // 45 / 41 / 51 / 67 on 30,000 x 4,000.
 template <typename T>
-static void forward_pick(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
+static const char *forward_pick(const LogitRows &in, const Targets &t, float inv_t, float *logprob, float *entropy, RowStats *stats,
                          hipStream_t stream) {
     const int32_t vectors = in.n / Elem<T>::kVec;
-    if (in.n <= kWaveRow) forward_rows<T, 64, 3>(in, t, inv_t, logprob, entropy, stats, stream);
-    else if (vectors < 2048) forward_rows<T, 256, 3>(in, t, inv_t, logprob, entropy, stats, stream);
-    else if (vectors < 12288) forward_rows<T, 512, 3>(in, t, inv_t, logprob, entropy, stats, stream);
-    else forward_rows<T, 1024, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (in.n <= kWaveRow) return forward_rows<T, 64, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (vectors < 2048) return forward_rows<T, 256, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    if (vectors < 12288) return forward_rows<T, 512, 3>(in, t, inv_t, logprob, entropy, stats, stream);
+    return forward_rows<T, 1024, 3>(in, t, inv_t, logprob, entropy, stats, stream);
 }
 
 template <typename T, int ROW, int UNROLL>
@@ -306,7 +308,7 @@ static const char *backward_launch(const LogitRows &in, const Targets &t, float 
     const int64_t per_tile = (int64_t)ROW * UNROLL * Elem<T>::kVec;
     const int64_t tiles = (in.n + per_tile - 1) / per_tile, per = 256 / ROW;
     const int64_t grid = (in.rows * tiles + per - 1) / per;
-    if (in.rows * tiles > 0x7FFFFFFF) return "too many elements for one launch";
+    if (in.rows * tiles > 0x7FFFFFFF || !launch_fits(grid, 256)) return "too many elements for one launch";
     typedef typename Elem<T>::Bits Bits;
     if (ge)
         hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
@@ -342,9 +344,12 @@ extern "C" int token_logprobs_forward_launcher(int64_t rows, int64_t n, int64_t 
     const Targets t = {target, target_bits == 64, ignore_index};
     const float inv_t = 1.f / temperature;
     hipStream_t s = (hipStream_t)stream;
-    if (type == kFp32) forward_pick<Single>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
-    else if (type == kFp16) forward_pick<Half>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
-    else forward_pick<BFloat16>(in, t, inv_t, (float *)logprob, (float *)entropy, (RowStats *)stats, s);
+    float *lp = (float *)logprob, *h = (float *)entropy;
+    RowStats *st = (RowStats *)stats;
+    const char *why = type == kFp32   ? forward_pick<Single>(in, t, inv_t, lp, h, st, s)
+                      : type == kFp16 ? forward_pick<Half>(in, t, inv_t, lp, h, st, s)
+                                      : forward_pick<BFloat16>(in, t, inv_t, lp, h, st, s);
+    if (why) return refuse(who, why);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }

@@ -43,6 +43,7 @@ class OpPolicyLoss(torch.autograd.Function):
                                   reduction, scratch, offsets, loss, stats)
         ctx.args = (reduction, offsets, entropy_coef, shape, logprob.dtype)
         ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)                # nothing is to be filled with zeros for the statistics
         ctx.save_for_backward(scratch, mask)
         return loss, stats
 

@@ -29,6 +29,7 @@ class OpPreferenceLoss(torch.autograd.Function):
                                       chosen, rejected)
         ctx.args = (offsets, shape, logprob.dtype)
         ctx.mark_non_differentiable(chosen, rejected)
+        ctx.set_materialize_grads(False)                # nothing is to be filled with zeros for the rewards
         ctx.save_for_backward(scratch, mask)
         return loss, chosen, rejected
 

@@ -48,6 +48,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
     if any(map(_is_none, grads)):
         outs = [o for g, o in zip(grads, outs) if g is not None]
         grads = [g for g in grads if g is not None]
+    if any(map(_is_none, outs)):
+        raise ValueError("a gradient without an output")
     if not (max_norm >= 0 and eps >= 0 and scale > 0 and math.isfinite(scale)):
         raise ValueError(f"max_norm and eps must not be negative and scale must be positive: {max_norm}, {eps}, {scale}")
     use_max = norm_type in ("inf", math.inf)

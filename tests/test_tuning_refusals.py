@@ -80,12 +80,17 @@ def logprobs(rows=2, n=8, inner=2, x=0x1000, code=0, target=0x2000, bits=64, tem
     C.token_logprobs_forward_launcher(rows, n, inner, 0, n, x, code, target, bits, -100, temperature, logprob, entropy, stats, 0)
 
 
+def test_clip_grads_without_an_output():
+    with pytest.raises(ValueError, match="without an output"):
+        clip_grads([torch.zeros(3)], 1.0, out=[None])
+
+
 def test_c_entries_refuse_on_the_host():
     logprobs(rows=0)
     for bad, text in (({"code": 3}, "type code"), ({"x": 0}, "null"), ({"target": 0}, "null"), ({"logprob": 0}, "null"), ({"bits": 16}, "bits"),
                       ({"x": 0x1002}, "aligned"), ({"target": 0x2004}, "aligned"), ({"stats": 0x4008}, "misaligned"),
                       ({"temperature": 0.0}, "temperature"), ({"temperature": math.nan}, "temperature"), ({"temperature": 1e-45}, "temperature"),
-                      ({"rows": 1 << 31}, "too many"), ({"n": 1 << 31}, "too many"), ({"inner": 0}, "too many")):
+                      ({"rows": 1 << 31}, "too many"), ({"n": 1 << 31}, "too many"), ({"rows": 1 << 26, "n": 5000}, "too many"), ({"inner": 0}, "too many")):
         with pytest.raises(RuntimeError, match=text):
             logprobs(**bad)
     with pytest.raises(RuntimeError, match="null"):
@@ -104,7 +109,8 @@ def test_policy_entry():
     for bad, text in (({"rows": -1}, "negative"), ({"reduction": 3}, "reduction"), ({"code": 7}, "type code"), ({"low": 1.5}, "clip"),
                       ({"high": math.nan}, "clip"), ({"dual": 0.5}, "dual_clip"), ({"loss": 0}, "null"), ({"weights": 0}, "null"),
                       ({"logprob": 0}, "null"), ({"logprob": 0x1002}, "misaligned"), ({"workspace": 0x5004}, "misaligned"), ({"col": 2}, "one to a"),
-                      ({"time": 1 << 31}, "too many"), ({"rows": 1 << 40}, "too many")):
+                      ({"time": 1 << 31}, "too many"), ({"rows": 1 << 40}, "too many"),
+                      ({"rows": 1 << 24, "time": 1 << 10}, "too many")):
         with pytest.raises(RuntimeError, match=text):
             policy(**bad)
     C.policy_loss_backward_launcher(0, 8, 0, 0, 0, 0, 0, 0, 0, 0.0, 0x1000, 0, 0)
@@ -122,7 +128,8 @@ def preference(pairs=2, time=8, code=0, logprob=0x1000, kind=0, beta=0.1, smooth
 def test_preference_entry():
     for bad, text in (({"pairs": -1}, "negative"), ({"kind": 3}, "kind"), ({"code": -1}, "type code"), ({"beta": 0.0}, "beta"),
                       ({"beta": math.inf}, "beta"), ({"smoothing": -0.1}, "smoothing"), ({"logprob": 0}, "null"), ({"slope": 0}, "null"),
-                      ({"chosen": 0x4002}, "misaligned"), ({"time": 1 << 31}, "too many"), ({"pairs": 1 << 31}, "too many")):
+                      ({"chosen": 0x4002}, "misaligned"), ({"time": 1 << 31}, "too many"), ({"pairs": 1 << 31}, "too many"),
+                      ({"pairs": 1 << 20, "time": 1 << 14}, "too many")):
         with pytest.raises(RuntimeError, match=text):
             preference(**bad)
     with pytest.raises(RuntimeError, match="null"):
