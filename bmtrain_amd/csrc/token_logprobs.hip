@@ -8,6 +8,9 @@
 // reads the logits once more and writes the gradient.  Both are bound by HBM (2 or 4 bytes per element read, and as
 // many written on the way back).
 //
+// The target is left out of the running sums and joins at the end: where it is the largest logit, logprob =
+// -log(1 + sum_{j != target} e^{z_j}) keeps its digits however near to 0 it is (as 1 - p does in the gradient), which a sum
+// of everything rounded at 1 would not.
 // (x_j - max) is formed before it is scaled: it is exact for neighbouring values, so rows of large magnitude lose
 // nothing, and a row of the type's lowest value gives z = 0 instead of inf - inf.  All sums and exponents are fp32; the
 // gradient is rounded once, to the logits' type.
@@ -72,6 +75,20 @@ __device__ __forceinline__ void online_join(Online &a, float m, float s, float w
     a.m = top;
 }
 
+// Element `at` of the vector becomes -inf.  And-or masks on whole words: written as a choice of elements it becomes an
+// indexed store to memory, which costs the kernel two fifths of its speed.
+template <typename T>
+__device__ __forceinline__ void leave_out(u32x4 &w, int at) {
+    constexpr int kPerWord = Elem<T>::kVec / 4;
+    const uint32_t shift = kPerWord == 2 ? 16u * (uint32_t)(at & 1) : 0u;
+    const uint32_t gone = (kPerWord == 2 ? 0xFFFFu : 0xFFFFFFFFu) << shift, put = (uint32_t)Elem<T>::put(-INFINITY) << shift;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t here = k == at / kPerWord ? 0xFFFFFFFFu : 0u;
+        w[k] = (w[k] & ~(gone & here)) | (put & here);
+    }
+}
+
 // K values x[0..K) into the running sums.
 template <bool ENTROPY, int K>
 __device__ __forceinline__ void online_add(Online &a, const float *x, float c) {
@@ -119,17 +136,26 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     const int nvec = (n - head) / E::kVec;
     const u32x4 *body = (const u32x4 *)(x + head);
     const float c = inv_t * kLog2e;
+    constexpr int K = E::kVec;
+    const bool inside = (uint64_t)t < (uint64_t)n;
     float xt = 0.f;
-    if (lane == 0 && (uint64_t)t < (uint64_t)n) xt = E::get(x[t]);
+    if (lane == 0 && inside) xt = E::get(x[t]);
+    // the vector that holds the target, in the lane that reads it, and the target's place in it; none in every other lane
+    const int body_t = inside ? (int)t - head : -1;
+    const int target_vec = body_t >= 0 && body_t / K < nvec && body_t / K % ROW == lane ? body_t / K : INT32_MIN, target_at = body_t % K;
 
     Online a = {-__FLT_MAX__, 0.f, 0.f};
-    constexpr int K = E::kVec;
     int i = lane;
     for (; i + (UNROLL - 1) * ROW < nvec; i += UNROLL * ROW) {
         u32x4 w[UNROLL];
         float v[UNROLL * K];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) w[u] = load_vector<PAST>(body + i + u * ROW);
+        if ((uint32_t)(target_vec - i) < (uint32_t)(UNROLL * ROW)) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++)
+                if (target_vec == i + u * ROW) leave_out<T>(w[u], target_at);
+        }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) E::unpack(w[u], v + u * K);
         online_add<ENTROPY, UNROLL * K>(a, v, c);
@@ -139,6 +165,11 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
 #pragma unroll
         for (int u = 0; u < UNROLL - 1; u++)
             if (i + u * ROW < nvec) w[u] = load_vector<PAST>(body + i + u * ROW);
+        if ((uint32_t)(target_vec - i) < (uint32_t)((UNROLL - 1) * ROW)) {
+#pragma unroll
+            for (int u = 0; u < UNROLL - 1; u++)
+                if (target_vec == i + u * ROW) leave_out<T>(w[u], target_at);
+        }
 #pragma unroll
         for (int u = 0; u < UNROLL - 1; u++) {
             if (i + u * ROW >= nvec) break;
@@ -149,7 +180,8 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     }
     const int tail_lo = head + nvec * K, edge = head + (n - tail_lo);      // fewer than 2 * kVec elements
     if (lane < edge) {
-        const float v = E::get(x[lane < head ? lane : tail_lo + (lane - head)]);
+        const int j = lane < head ? lane : tail_lo + (lane - head);
+        const float v = j == t ? -INFINITY : E::get(x[j]);
         online_add<ENTROPY, 1>(a, &v, c);
     }
 #pragma unroll
@@ -165,9 +197,20 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
         for (int k = 1; k < WAVES; k++) online_join<ENTROPY>(a, part[k].m, part[k].s, part[k].w, c);
     }
     if (lane == 0) {
-        const float log_sum = logf(a.s);
+        float log_sum, lp = __builtin_nanf("");
+        if (inside && xt >= a.m) {                        // z = 0 for the target, all others together weigh `rest`
+            const float d = (a.m - xt) * c, f = __builtin_amdgcn_exp2f(d), rest = a.s * f;
+            if (ENTROPY) a.w = __builtin_fmaf(fmaxf(d, kFar), a.s, a.w) * f;
+            a.m = xt, a.s = 1.f + rest;
+            log_sum = log1pf(rest);
+            lp = (xt - xt) - log_sum;                     // NaN for an infinite logit
+        } else {
+            if (inside) online_join<ENTROPY>(a, xt, 1.f, 0.f, c);
+            log_sum = logf(a.s);
+            if (inside) lp = (xt - a.m) * inv_t - log_sum;
+        }
         const float h = ENTROPY ? log_sum - kLn2 * (a.w / a.s) : 0.f;
-        logprob[r] = (uint64_t)t < (uint64_t)n ? (xt - a.m) * inv_t - log_sum : __builtin_nanf("");
+        logprob[r] = lp;
         if (ENTROPY) entropy[r] = h;
         if (stats) stats[r] = RowStats{a.m, log_sum, h, 0.f};
     }
@@ -203,11 +246,15 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
     const RowStats st = live ? stats[r] : RowStats{0.f, 0.f, 0.f, 0.f};
     // p = 2^y with y = (x - max) * c - log2(sum), log p = y ln 2:  dx = p (a + b y), a = -(g + h H) / T, b = -h ln 2 / T
     const float c = inv_t * kLog2e, log2_sum = st.log_sum * kLog2e;
-    const float hot = g * inv_t, b = -h * inv_t * kLn2, a = -(g + h * st.entropy) * inv_t;
+    const float hot = g * inv_t, b = -h * inv_t * kLn2, a_rest = -h * st.entropy * inv_t, a = a_rest - hot;
     auto one = [&](float v) {
         const float y = __builtin_fmaf(v - st.max, c, -log2_sum);
         const float p = __builtin_amdgcn_exp2f(y);
         return p * (ENTROPY ? __builtin_fmaf(b, fmaxf(y, kFar), a) : a);
+    };
+    auto target_one = [&](float v) {                      // the same with (1 - p) g / T in the place of g / T - p g / T
+        const float y = __builtin_fmaf(v - st.max, c, -log2_sum);
+        return __builtin_fmaf(__builtin_amdgcn_exp2f(y), __builtin_fmaf(b, fmaxf(y, kFar), a_rest), -expm1f(y * kLn2) * hot);
     };
     const int i0 = tile * (ROW * UNROLL) + lane;
     u32x4 w[UNROLL];
@@ -222,15 +269,22 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
         if (i >= nvec) break;
         u32x4 packed = {0u, 0u, 0u, 0u};
         if (live) {
-            float v[K];
+            float v[K], x_target = 0.f;
             E::unpack(w[u], v);
-#pragma unroll
-            for (int k = 0; k < K; k++) v[k] = one(v[k]);
             const int64_t at = t - (head + (int64_t)i * K);
-            if ((uint64_t)at < (uint64_t)K) {
+            const bool has_target = (uint64_t)at < (uint64_t)K;
+            if (has_target) {
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    if (k == (int)at) v[k] += hot;
+                    if (k == (int)at) x_target = v[k];
+            }
+#pragma unroll
+            for (int k = 0; k < K; k++) v[k] = one(v[k]);
+            if (has_target) {
+                x_target = target_one(x_target);
+#pragma unroll
+                for (int k = 0; k < K; k++)
+                    if (k == (int)at) v[k] = x_target;
             }
             packed = E::pack(v);
         }
@@ -241,8 +295,8 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
         const int j = lane < head ? lane : tail_lo + (lane - head);
         float v = 0.f;
         if (live) {
-            v = one(E::get(x[j]));
-            if (j == t) v += hot;
+            v = E::get(x[j]);
+            v = j == t ? target_one(v) : one(v);
         }
         d[j] = E::put(v);
     }

@@ -300,3 +300,32 @@ def test_side_stream_and_graph():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), seed
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 257, 4999, 33000])
+def test_confident_tokens_keep_their_digits(dtype, n):
+    """The target far above everything else: log-probabilities of 1e-2 .. 1e-30 and the gradient 1 - p, relative to
+    themselves.  The others' sum has at most 64 additions and exponentials of |z| <= R: (64 + 8 R) u relative, and half
+    as much again for its logarithm and the products."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    lifts = torch.tensor([6.0, 14.0, 20.0, 34.0, 60.0], device="cuda")
+    logits = (torch.randn(5, n, generator=gen, device="cuda") * 0.5).clamp(-2, 2)
+    target = torch.randint(0, n, (5,), generator=gen, device="cuda")
+    logits[torch.arange(5), target] = lifts + 2
+    logits = logits.to(dtype)
+    leaf = logits.clone().requires_grad_()
+    logp, entropy = TokenLogProbs(entropy=True)(leaf, target)
+    grad, = torch.autograd.grad((logp, entropy), leaf, (torch.ones(5, device="cuda"), torch.zeros(5, device="cuda")))
+    x = logits.double()
+    others = x - x.gather(1, target.unsqueeze(1))
+    rest = others.exp().scatter(1, target.unsqueeze(1), 0.0).sum(1)
+    want = -torch.log1p(rest)
+    tol = U * 1.5 * (64 + 8 * 66) * 2
+    assert ((logp.double() - want).abs() <= tol * want.abs()).all()
+    weighted = (others * others.exp()).scatter(1, target.unsqueeze(1), 0.0).sum(1)
+    want_entropy = torch.log1p(rest) - weighted / (1 + rest)
+    assert ((entropy.double() - want_entropy).abs() <= 4 * tol * want_entropy).all()
+    at_target = grad.double().gather(1, target.unsqueeze(1)).squeeze(1)
+    tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126, torch.float32: 2.0 ** -126}[dtype]
+    assert ((at_target - rest / (1 + rest)).abs() <= (tol + torch.finfo(dtype).eps / 2 * 1.01) * rest + tiny).all()
