@@ -222,14 +222,19 @@ def _codes(tensors):
 
 def clip_table(grads, outs=None):
     """``C.clip_table`` of dense GPU tensors of fp32, fp16 or bf16 on one device; ``outs`` (default: the gradients
-    themselves) have their gradients' numbers of elements, and their strides where a gradient is not contiguous.  Every
-    property is read once for the whole list: with many small gradients this is what a call costs."""
+    themselves) have their gradients' numbers of elements, and their strides where a gradient is not contiguous.  With
+    many small gradients this is what a call costs: lists of contiguous tensors are read by the library, anything else
+    (and what is to be refused) here, every property once for the whole list."""
+    outs = grads if outs is None else outs
+    read = C.clip_table_from_tensors(grads, outs)
+    if read is not None:
+        return read[0]
     codes = _codes(grads)
     sources = list(map(_Tensor.data_ptr, grads))
     counts = list(map(_Tensor.numel, grads))
     devices = set(map(_Tensor.get_device, grads))
     dense = all(map(_Tensor.is_contiguous, grads))
-    if outs is None or outs is grads:
+    if outs is grads:
         out_codes, destinations = codes, sources
         assert dense or all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
     else:

@@ -10,10 +10,6 @@ from ..loss._function import on_device_of
 from . import _function as F
 
 
-def _is_none(t):
-    return t is None
-
-
 
 @torch.no_grad()
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, eps: float = 1e-6, scale: float = 1.0,
@@ -45,10 +41,11 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(outs)} outputs")
-    if any(map(_is_none, grads)):
+    if type(None) in set(map(type, grads)):
         outs = [o for g, o in zip(grads, outs) if g is not None]
         grads = [g for g in grads if g is not None]
-    if any(map(_is_none, outs)):
+        outs = grads if out is None else outs
+    if type(None) in set(map(type, outs)):
         raise ValueError("a gradient without an output")
     if not (max_norm >= 0 and eps >= 0 and scale > 0 and math.isfinite(scale)):
         raise ValueError(f"max_norm and eps must not be negative and scale must be positive: {max_norm}, {eps}, {scale}")

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from bmtrain_amd import C
 from bmtrain_amd.optim import OptimManager, clip_grads, _function as OF
 
 pytestmark = pytest.mark.gpu
@@ -220,6 +221,25 @@ def test_manager_scales_with_the_same_bits(dtypes):
         norm = manager.clip_grad_norm([{"params": [twice, twice]}], max_norm)
         coef = float(max_norm * 8.0) / (norm * 8.0 + 1e-6)
         assert torch.equal(twice.grad, b.mul_(coef).mul_(coef) if coef < 1 else b)
+
+
+def test_both_ways_of_reading_tensors_agree(monkeypatch):
+    """The table the library reads by itself against the one built property by property; lists it does not take."""
+    base = torch.randn(7, 11, device="cuda")
+    grads = [base, base[2:5], torch.empty(0, 3, device="cuda"), torch.nn.Parameter(torch.zeros(5, device="cuda")), torch.zeros((), device="cuda"),
+             torch.zeros(6, device="cuda", requires_grad=True), base[1:2, :].t(), base.bfloat16()[:, :], torch.zeros(9, device="cuda").half()]
+    outs = [torch.empty_like(g, dtype=torch.bfloat16) for g in grads]
+    read = C.clip_table_from_tensors(grads, outs)
+    if read is None:
+        pytest.skip("this torch offers no DLPack exchange table")
+    read_in_place = C.clip_table_from_tensors(grads, grads)
+    for bad in ([base.t()], [base[:, 1:]], [base.double()], [base.cpu()], [base.int()], [base.to(torch.complex64)]):
+        assert C.clip_table_from_tensors(bad, bad) is None
+    assert C.clip_table_from_tensors([base], [base[1:]]) is None
+    monkeypatch.setattr(C, "_read_tensor", None)
+    assert C.clip_table_from_tensors(grads, outs) is None
+    assert read == (OF.clip_table(grads, outs), 0) and read_in_place == (OF.clip_table(grads), 0)
+    check([base.clone(), base.bfloat16()], 0.3, out=[torch.empty_like(base), torch.empty_like(base).half()])
 
 
 def test_autograd_notices_the_write():

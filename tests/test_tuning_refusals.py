@@ -80,6 +80,17 @@ def logprobs(rows=2, n=8, inner=2, x=0x1000, code=0, target=0x2000, bits=64, tem
     C.token_logprobs_forward_launcher(rows, n, inner, 0, n, x, code, target, bits, -100, temperature, logprob, entropy, stats, 0)
 
 
+def test_tensors_read_by_the_library():
+    """Lists it does not take (on the CPU, strided, of other types) are left to the slower reading, without an error."""
+    cpu = [torch.zeros(3), torch.zeros(4, requires_grad=True)]
+    assert C.clip_table_from_tensors(cpu, cpu) is None
+    assert C.clip_table_from_tensors([], []) is None
+    assert C.clip_table_from_tensors([1.0], [1.0]) is None
+    assert C.clip_table_from_tensors([None], [None]) is None
+    assert C.clip_table_from_tensors([torch.zeros(2, 3).t()], [torch.zeros(6)]) is None
+    assert C.clip_table_from_tensors([torch.zeros(3, dtype=torch.complex64).conj()], [torch.zeros(3)]) is None
+
+
 def test_clip_grads_without_an_output():
     with pytest.raises(ValueError, match="without an output"):
         clip_grads([torch.zeros(3)], 1.0, out=[None])
