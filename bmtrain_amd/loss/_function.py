@@ -166,6 +166,10 @@ def on_device_of(t: torch.Tensor):
     return _HERE if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
 
 
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _dense(name: str, t, device: int, dtype: torch.dtype, numel: int) -> int:
     """Pointer of a contiguous tensor of `numel` elements on `device`; 0 for None."""
     if t is None:
@@ -245,7 +249,7 @@ def _tokens(name: str, t, shape, dtype, device: int):
 
 def _mask(mask, shape, device: int):
     if mask is None:
-        return 0, 0
+        return 0, 0                                     # every token counts
     assert mask.dtype in _MASK_TYPES, "mask must be a bool or uint8 tensor"
     return _tokens("mask", mask, shape, mask.dtype, device)
 
@@ -279,15 +283,15 @@ def policy_loss_forward(logprob, old_logprob, ref_logprob, entropy, advantages, 
         assert advantages.get_device() == device, "advantages must be on the same cuda device as the other tensors"
         advantage, advantage_row, per_token = advantages.data_ptr(), advantages.stride(0), 0
     floats, weights, saved = offsets
-    base = _dense("scratch", scratch, device, torch.float32, floats)
+    assert scratch.numel() == floats, "scratch must be what policy_loss_scratch says"
+    base = scratch.data_ptr()
     C.policy_loss_forward_launcher(rows, time, code, *_tokens("logprob", logprob, shape, dtype, device),
                                    *_tokens("old_logprob", old_logprob, shape, dtype, device),
                                    *_tokens("ref_logprob", ref_logprob, shape, dtype, device),
                                    *_tokens("entropy", entropy, shape, dtype, device), advantage, advantage_row, per_token,
                                    *_mask(mask, shape, device), clip_low, clip_high, dual_clip, kl_coef, entropy_coef, reduction,
-                                   base + 4 * saved if saved >= 0 else 0, base + 4 * weights, base,
-                                   _dense("loss", loss, device, torch.float32, 1),
-                                   _dense("stats", stats, device, torch.float32, 5), _stream_of(device))
+                                   base + 4 * saved if saved >= 0 else 0, base + 4 * weights, base, loss.data_ptr(),
+                                   stats.data_ptr(), _stream_of(device))
 
 
 def policy_loss_backward(reduction: int, scratch, offsets, upstream, mask, entropy_coef: float, grad_logprob, grad_entropy) -> None:
@@ -295,16 +299,14 @@ def policy_loss_backward(reduction: int, scratch, offsets, upstream, mask, entro
     first = grad_logprob if grad_logprob is not None else grad_entropy
     if first is None:
         return
-    device, shape, dtype = first.get_device(), first.shape, first.dtype
+    device, shape = first.get_device(), first.shape
     floats, weights, saved = offsets
-    assert saved >= 0 or grad_logprob is None, "the forward call kept no derivatives"
-    base = _dense("scratch", scratch, device, torch.float32, floats)
-    n = shape[0] * shape[1]
-    C.policy_loss_backward_launcher(*shape, _type_code("policy_loss", dtype), reduction, base + 4 * saved if saved >= 0 else 0,
-                                    base + 4 * weights, _dense("upstream", upstream, device, torch.float32, 1),
-                                    *_mask(mask, shape, device), entropy_coef,
-                                    _dense("grad_logprob", grad_logprob, device, dtype, n),
-                                    _dense("grad_entropy", grad_entropy, device, dtype, n), _stream_of(device))
+    assert scratch.numel() == floats and (saved >= 0 or grad_logprob is None), "scratch must be that of the forward call"
+    assert upstream.get_device() == device and upstream.dtype == torch.float32 and upstream.numel() == 1, "upstream must be one float on cuda"
+    base = scratch.data_ptr()
+    C.policy_loss_backward_launcher(*shape, _TYPE_CODES[first.dtype], reduction, base + 4 * saved if saved >= 0 else 0,
+                                    base + 4 * weights, upstream.data_ptr(), *((0, 0) if mask is None else (mask.data_ptr(), mask.stride(0))),
+                                    entropy_coef, _ptr(grad_logprob), _ptr(grad_entropy), _stream_of(device))
 
 
 def preference_loss_scratch(pairs: int, time: int):
@@ -324,22 +326,21 @@ def preference_loss_forward(logprob, ref_logprob, mask, kind: int, average: bool
     code = _type_code("preference_loss", dtype)
     pairs = shape[0] // 2
     floats, slope = offsets
-    base = _dense("scratch", scratch, device, torch.float32, floats)
+    assert scratch.numel() == floats, "scratch must be what preference_loss_scratch says"
+    base = scratch.data_ptr()
     C.preference_loss_forward_launcher(pairs, shape[1], code, *_tokens("logprob", logprob, shape, dtype, device),
                                        *_tokens("ref_logprob", ref_logprob, shape, dtype, device), *_mask(mask, shape, device),
-                                       kind, int(average), beta, label_smoothing, base,
-                                       _dense("loss", loss, device, torch.float32, 1),
-                                       _dense("chosen", chosen, device, torch.float32, pairs),
-                                       _dense("rejected", rejected, device, torch.float32, pairs), base + 4 * slope,
-                                       _stream_of(device))
+                                       kind, int(average), beta, label_smoothing, base, loss.data_ptr(), chosen.data_ptr(),
+                                       rejected.data_ptr(), base + 4 * slope, _stream_of(device))
 
 
 def preference_loss_backward(scratch, offsets, upstream, mask, grad_logprob) -> None:
     """Gradient (contiguous [2 * pairs, time]) of ``preference_loss_forward``."""
-    device, shape = grad_logprob.get_device(), grad_logprob.shape
+    rows, time = grad_logprob.shape
     floats, slope = offsets
-    C.preference_loss_backward_launcher(shape[0] // 2, shape[1], _type_code("preference_loss", grad_logprob.dtype),
-                                        _dense("scratch", scratch, device, torch.float32, floats) + 4 * slope,
-                                        _dense("upstream", upstream, device, torch.float32, 1), *_mask(mask, shape, device),
-                                        _dense("grad_logprob", grad_logprob, device, grad_logprob.dtype, shape[0] * shape[1]),
-                                        _stream_of(device))
+    assert scratch.numel() == floats, "scratch must be that of the forward call"
+    device = grad_logprob.get_device()
+    assert upstream.get_device() == device and upstream.dtype == torch.float32 and upstream.numel() == 1, "upstream must be one float on cuda"
+    C.preference_loss_backward_launcher(rows // 2, time, _TYPE_CODES[grad_logprob.dtype], scratch.data_ptr() + 4 * slope,
+                                        upstream.data_ptr(), *((0, 0) if mask is None else (mask.data_ptr(), mask.stride(0))),
+                                        grad_logprob.data_ptr(), _stream_of(device))

@@ -53,8 +53,9 @@ class OpPolicyLoss(torch.autograd.Function):
         scratch, mask = ctx.saved_tensors
         reduction, offsets, entropy_coef, shape, dtype = ctx.args
         with F.on_device_of(scratch):
-            grad_logprob, grad_entropy = [torch.empty(shape, device=scratch.device, dtype=dtype) if needed else None
-                                          for needed in ctx.needs_input_grad[:2]]
+            device = scratch.device
+            grad_logprob = torch.empty(shape, device=device, dtype=dtype) if ctx.needs_input_grad[0] else None
+            grad_entropy = torch.empty(shape, device=device, dtype=dtype) if ctx.needs_input_grad[1] else None
             F.policy_loss_backward(reduction, scratch, offsets, upstream, mask, entropy_coef, grad_logprob, grad_entropy)
         return grad_logprob, grad_entropy, None, None, None, None, None, None, None, None
 
@@ -111,10 +112,7 @@ class PolicyLoss(torch.nn.Module):
             advantages = advantages[:, 0]              # one to a sequence: [sequences, 1], or an expanded view
         if advantages.dtype != torch.float32:
             advantages = advantages.float()
-        if advantages.dim() == 1:
-            advantages = advantages.detach() if advantages.requires_grad else advantages
-        else:
-            advantages = constant(advantages)
+        advantages = constant(advantages) if advantages.dim() == 2 else advantages.detach() if advantages.requires_grad else advantages
         return OpPolicyLoss.apply(_tokens_adjacent(logprob), _tokens_adjacent(entropy), constant(old_logprob), advantages,
                                   as_mask(mask), constant(ref_logprob),
                                   (self.clip_low, self.clip_high, self.dual_clip or 0.0), self.kl_coef, self.entropy_coef,
