@@ -150,7 +150,9 @@ _tensor_types = {_torch.Tensor, _torch.nn.Parameter}
 def clip_table_from_tensors(sources: list, destinations: list):
     """(`bmt_clip_tensor` array, device) of two lists of contiguous GPU tensors (the same list twice: in place), read by the
     library itself; None where they are not all of that kind, or torch does not offer the means."""
-    if _read_tensor is None or not sources or not (set(map(type, sources)) | set(map(type, destinations))) <= _tensor_types:
+    if _read_tensor is None or not sources or type(sources) is not list or type(destinations) is not list:
+        return None
+    if len(sources) != len(destinations) or not (set(map(type, sources)) | set(map(type, destinations))) <= _tensor_types:
         return None
     table = array.array("q", bytes(32 * len(sources)))
     device = _i32()

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
                 }
                 const float r = over ? (A > 0.f ? in.ratio_high : in.ratio_far) : under ? in.ratio_low : 1.f + rm1;
                 const float policy = -r * A;
-                const float slope = __builtin_fmaf(-in.kl_coef, qm1, over || under ? 0.f : policy);
+                const float slope = (over || under ? 0.f : policy) - (in.kl_coef != 0.f ? in.kl_coef * qm1 : 0.f);
                 const bool on = mask_set(now.mask, k);
                 g[k] = on ? slope : 0.f;
                 sum[0] += on ? policy : 0.f;
@@ -235,7 +235,8 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
     if (threadIdx.x == 0) {
         const double share = reduction == kSum ? 1.0 : all[5] > 0 ? 1.0 / all[5] : 0.0;     // nothing counts: loss 0
         for (int k = 0; k < 5; k++) all[k] *= share;
-        loss[0] = (float)(all[0] + (double)kl_coef * all[1] - (double)entropy_coef * all[2]);
+        // a term without weight is only measured: no 0 * inf
+        loss[0] = (float)(all[0] + (kl_coef != 0.f ? (double)kl_coef * all[1] : 0.0) - (entropy_coef != 0.f ? (double)entropy_coef * all[2] : 0.0));
         for (int k = 0; k < 5; k++) stats[k] = (float)all[k];
         weights[0] = (float)share;
     }

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
         float v[UNROLL * K];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) w[u] = load_vector<PAST>(body + i + u * ROW);
-        if ((uint32_t)(target_vec - i) < (uint32_t)(UNROLL * ROW)) {
+        if ((uint32_t)target_vec - (uint32_t)i < (uint32_t)(UNROLL * ROW)) {
 #pragma unroll
             for (int u = 0; u < UNROLL; u++)
                 if (target_vec == i + u * ROW) leave_out<T>(w[u], target_at);
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
 #pragma unroll
         for (int u = 0; u < UNROLL - 1; u++)
             if (i + u * ROW < nvec) w[u] = load_vector<PAST>(body + i + u * ROW);
-        if ((uint32_t)(target_vec - i) < (uint32_t)((UNROLL - 1) * ROW)) {
+        if ((uint32_t)target_vec - (uint32_t)i < (uint32_t)((UNROLL - 1) * ROW)) {
 #pragma unroll
             for (int u = 0; u < UNROLL - 1; u++)
                 if (target_vec == i + u * ROW) leave_out<T>(w[u], target_at);

@@ -76,7 +76,7 @@ class PolicyLoss(torch.nn.Module):
     Args:
         clip_low, clip_high: the clip range around 1 (``clip_high`` defaults to ``clip_low``).
         dual_clip: bound for negative advantages, above 1; None for none.
-        kl_coef, entropy_coef: weights of the terms.
+        kl_coef, entropy_coef: weights of the terms; a term of weight 0 is only measured, one without its input is 0.
         reduction: R is ``'mean'``: the mean over all tokens under the mask, ``'sequence'``: the mean over the sequences
             with at least one such token of their own means, ``'sum'``: the sum.  With nothing under the mask R is 0.
 

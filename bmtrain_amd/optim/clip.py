@@ -59,6 +59,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         result = torch.empty(2, dtype=torch.float32, device=grads[0].device)
         F.grad_norm_multi(table, use_max, float(max_norm), float(eps), float(scale), result)
         F.grad_scale_multi(table, result[1])
-    if not torch.is_inference_mode_enabled():
+    try:
         torch.autograd.graph.increment_version(outs)        # autograd is to notice the write, as with any in-place operation
+    except RuntimeError:                                    # inference tensors: nothing keeps them for a backward pass
+        pass
     return result[0]

@@ -251,6 +251,14 @@ def test_autograd_notices_the_write():
         y.backward()
 
 
+def test_inference_tensors():
+    with torch.inference_mode():
+        g = grads_of([1000], (torch.float32,), 3)
+        check(g, 0.1)
+    check([g[0]], 0.05, out=[torch.empty_like(g[0])])
+    clip_grads(g, 0.01)
+
+
 def test_a_larger_grid_than_one_batch_of_every_type():
     """More tensors than a launch takes, types mixed, outputs of mixed types."""
     sizes = [(k * 37) % 999 + 1 for k in range(500)]

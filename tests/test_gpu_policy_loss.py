@@ -179,6 +179,20 @@ def test_borders_of_the_clips_are_decided_on_the_exact_difference():
     assert torch.equal(grad != 0, inside) and stats[3] == float((~inside).sum())
 
 
+def test_terms_without_weight_are_only_measured():
+    """kl_coef and entropy_coef 0: an infinite KL or entropy shows in the statistics and nowhere else."""
+    data = make(4, 300, torch.float32, 9)
+    data["mask"][:, 0] = True
+    plain = check({**data, "ref": None, "entropy": None}, reduction="sequence")
+    data["ref"][1, 0] = 200.0
+    data["entropy"][2, 0] = float("inf")
+    leaf = data["logprob"].clone().requires_grad_()
+    loss, stats = PolicyLoss(reduction="sequence")(leaf, data["old"], data["advantages"], data["mask"], data["ref"], data["entropy"])
+    grad, = torch.autograd.grad(loss, leaf, torch.tensor(3.0, device="cuda"))
+    assert torch.equal(loss, plain[0]) and torch.equal(grad, plain[2])
+    assert stats[1] == float("inf") and stats[2] == float("inf")
+
+
 def test_small_kl_keeps_its_digits():
     """q around 1e-3 .. 1e-6: e^q - 1 - q = q^2 / 2 (1 + q / 3 + ...), where the plain difference has lost everything."""
     new = torch.full((1, 64), -0.5, device="cuda")

@@ -89,6 +89,10 @@ def test_tensors_read_by_the_library():
     assert C.clip_table_from_tensors([None], [None]) is None
     assert C.clip_table_from_tensors([torch.zeros(2, 3).t()], [torch.zeros(6)]) is None
     assert C.clip_table_from_tensors([torch.zeros(3, dtype=torch.complex64).conj()], [torch.zeros(3)]) is None
+    assert C.clip_table_from_tensors((torch.zeros(3),), (torch.zeros(3),)) is None
+    assert C.clip_table_from_tensors([torch.zeros(3)], []) is None
+    with pytest.raises((RuntimeError, ValueError, BufferError, AssertionError)):
+        clip_grads([torch.zeros(3).to_sparse()], 1.0)
 
 
 def test_clip_grads_without_an_output():
