@@ -216,19 +216,16 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
     }
 }
 
-// Workgroups of consecutive tiles on one XCD: 32 against one, two vectors to a lane in both: 664 / 697 us on 8,192 x 128,256
-// bf16 with entropies, 326 / 334 on 16,384 x 32,000 fp16 (6.4 TB/s); 16 to 128 measure alike, 4 and 512 are slower.
-constexpr uint32_t kBackwardRun = 32;
-
-// A tile is UNROLL vectors of ROW lanes; tiles are numbered through the rows.
+// A tile is UNROLL vectors of ROW lanes; tiles are numbered through the rows, and every XCD works on runs of consecutive
+// ones, 32 workgroups of 256 or 8 of 1,024.
 template <typename T, int ROW, int UNROLL, bool ENTROPY>
-__global__ __launch_bounds__(256) void token_logprobs_backward_kernel(
+__global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_backward_kernel(
     LogitRows in, Targets target, float inv_t, const RowStats *__restrict__ stats, const float *__restrict__ grad_logprob,
     const float *__restrict__ grad_entropy, typename Elem<T>::Bits *__restrict__ grad, int32_t tiles) {
     typedef Elem<T> E;
-    constexpr int PER = 256 / ROW, K = E::kVec;
+    constexpr int PER = ROW < 256 ? 256 / ROW : 1, K = E::kVec;
     const int lane = threadIdx.x % ROW;
-    const uint32_t unit = xcd_run<kBackwardRun>(blockIdx.x, gridDim.x) * PER + threadIdx.x / ROW;
+    const uint32_t unit = xcd_run<(ROW > 256 ? 8 : 32)>(blockIdx.x, gridDim.x) * PER + threadIdx.x / ROW;
     const int32_t r = (int32_t)(unit / (uint32_t)tiles), tile = (int32_t)(unit - (uint32_t)r * (uint32_t)tiles);
     if (PER > 1 && r >= in.rows) return;
     const int64_t t = target.at(r);
@@ -359,16 +356,17 @@ static const char *forward_pick(const LogitRows &in, const Targets &t, float inv
 template <typename T, int ROW, int UNROLL>
 static const char *backward_launch(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
                                    const float *ge, void *grad, hipStream_t stream) {
+    constexpr unsigned threads = ROW < 256 ? 256 : ROW;
     const int64_t per_tile = (int64_t)ROW * UNROLL * Elem<T>::kVec;
-    const int64_t tiles = (in.n + per_tile - 1) / per_tile, per = 256 / ROW;
+    const int64_t tiles = (in.n + per_tile - 1) / per_tile, per = ROW < 256 ? 256 / ROW : 1;
     const int64_t grid = (in.rows * tiles + per - 1) / per;
-    if (in.rows * tiles > 0x7FFFFFFF || !launch_fits(grid, 256)) return "too many elements for one launch";
+    if (in.rows * tiles > 0x7FFFFFFF || !launch_fits(grid, threads)) return "too many elements for one launch";
     typedef typename Elem<T>::Bits Bits;
     if (ge)
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(threads), 0, stream, in, t, inv_t,
                            stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     else
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, false>), dim3((unsigned)grid), dim3(256), 0, stream, in, t, inv_t,
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, false>), dim3((unsigned)grid), dim3(threads), 0, stream, in, t, inv_t,
                            stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     return nullptr;
 }
@@ -376,9 +374,13 @@ template <typename T>
 static const char *backward_pick(const LogitRows &in, const Targets &t, float inv_t, const RowStats *stats, const float *gl,
                                  const float *ge, void *grad, hipStream_t stream) {
     if (in.n <= kWaveRow) return backward_launch<T, 64, 4>(in, t, inv_t, stats, gl, ge, grad, stream);
-    // two vectors to a lane where a row has four such tiles or more (664 us against 683 with four on 8,192 x 128,256 bf16);
-    // a shorter row leaves much of its last tile idle and needs more in flight (20,000 x 5,000 fp16: 83 us with two, 67)
-    if (in.n > 4 * 512 * Elem<T>::kVec) return backward_launch<T, 256, 2>(in, t, inv_t, stats, gl, ge, grad, stream);
+    // Tiles of 2,048 vectors where they leave at most 15 % of a row's last one idle, of 512 where a row has four of those, of
+    // 1,024 in rows shorter than that.  Measured (us; 2,048 / 512 / 1,024): 8,192 x 128,256 bf16 with entropies 661 / 692 /
+    // 710, 16,384 x 32,000 fp16 329 / 344 / 365, 2,049 x 50,257 fp32 129 / 137 / 138; 5,000 x 20,000 bf16 (61 % full) 76 /
+    // 67; 20,000 x 5,000 fp16 - / 83 / 67.  Without runs of tiles on one XCD 697 and 334 (tiles of 512).
+    const int64_t vectors = in.n / Elem<T>::kVec, large = (vectors + 2047) / 2048 * 2048;
+    if (vectors * 100 >= large * 85) return backward_launch<T, 1024, 2>(in, t, inv_t, stats, gl, ge, grad, stream);
+    if (vectors > 4 * 512) return backward_launch<T, 256, 2>(in, t, inv_t, stats, gl, ge, grad, stream);
     return backward_launch<T, 256, 4>(in, t, inv_t, stats, gl, ge, grad, stream);
 }
 
