@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_backward_kernel(
         const uint32_t m = load_mask4(mask ? mask + row * mask_row + i : nullptr, count);
         float g[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) g[k] = mask_set(m, k) ? -entropy_coef * scale : 0.f;
+        for (int k = 0; k < 4; k++) g[k] = mask_set(m, k) && entropy_coef != 0.f ? -entropy_coef * scale : 0.f;
         store4<T>(grad_entropy + at, count, g);
     }
 }

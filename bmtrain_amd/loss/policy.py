@@ -50,6 +50,8 @@ class OpPolicyLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, _):
+        if upstream is None:
+            return (None,) * 10
         scratch, mask = ctx.saved_tensors
         reduction, offsets, entropy_coef, shape, dtype = ctx.args
         with F.on_device_of(scratch):
@@ -107,7 +109,7 @@ class PolicyLoss(torch.nn.Module):
                 mask: Optional[torch.Tensor] = None, ref_logprob: Optional[torch.Tensor] = None,
                 entropy: Optional[torch.Tensor] = None):
         assert logprob.dim() == 2, "logprob must be [sequences, tokens]"
-        if advantages.dim() == 2 and advantages.size(0) and (advantages.shape != logprob.shape or advantages.stride(1) == 0):
+        if advantages.dim() == 2 and advantages.size(1) and (advantages.shape != logprob.shape or advantages.stride(1) == 0):
             assert advantages.size(1) == 1 or advantages.shape == logprob.shape, "advantages must be one to a sequence or one to a token"
             advantages = advantages[:, 0]              # one to a sequence: [sequences, 1], or an expanded view
         if advantages.dtype != torch.float32:

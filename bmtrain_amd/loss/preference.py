@@ -36,6 +36,8 @@ class OpPreferenceLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, *_):
+        if upstream is None:
+            return (None,) * 7
         scratch, mask = ctx.saved_tensors
         offsets, shape, dtype = ctx.args
         with F.on_device_of(scratch):

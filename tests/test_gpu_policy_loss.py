@@ -191,6 +191,30 @@ def test_terms_without_weight_are_only_measured():
     grad, = torch.autograd.grad(loss, leaf, torch.tensor(3.0, device="cuda"))
     assert torch.equal(loss, plain[0]) and torch.equal(grad, plain[2])
     assert stats[1] == float("inf") and stats[2] == float("inf")
+    entropy = data["entropy"].clone().requires_grad_()
+    loss, _ = PolicyLoss()(data["logprob"], data["old"], data["advantages"], data["mask"], entropy=entropy)
+    grad, = torch.autograd.grad(loss, entropy, torch.tensor(float("inf"), device="cuda"))
+    assert (grad == 0).all()
+
+
+class Stop(torch.autograd.Function):
+    """Hands no gradient on, not even zeros."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, upstream):
+        return None
+
+
+def test_no_gradient_from_behind():
+    data = make(3, 50, torch.float32, 4)
+    leaf = data["logprob"].clone().requires_grad_()
+    loss, _ = PolicyLoss()(leaf, data["old"], data["advantages"], data["mask"])
+    Stop.apply(loss).backward()
+    assert leaf.grad is None or (leaf.grad == 0).all()
 
 
 def test_small_kl_keeps_its_digits():
@@ -259,6 +283,10 @@ def test_empty_batches():
             assert loss == 0 and (stats == 0).all()
             grad, = torch.autograd.grad(loss, leaf)
             assert grad.shape == shape
+            one_each = torch.zeros(shape[0], 1, device="cuda")
+            for advantages in (one_each, one_each.expand(shape), torch.zeros(shape, device="cuda")):
+                loss, stats = PolicyLoss(reduction=reduction)(leaf, leaf.detach(), advantages)
+                assert loss == 0 and (stats == 0).all()
 
 
 def test_gradient_against_differences():

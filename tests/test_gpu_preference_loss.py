@@ -133,6 +133,24 @@ def test_sums_per_row_and_layouts():
         assert grad.shape == shape
 
 
+class Stop(torch.autograd.Function):
+    """Hands no gradient on, not even zeros."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, upstream):
+        return None
+
+
+def test_no_gradient_from_behind():
+    leaf = torch.zeros(4, 6, device="cuda", requires_grad=True)
+    Stop.apply(PreferenceLoss()(leaf)[0]).backward()
+    assert leaf.grad is None or (leaf.grad == 0).all()
+
+
 def test_gradient_against_differences():
     logprob, ref, mask = make(4, 30, torch.float32, 12)
     for kind in ("sigmoid", "ipo"):

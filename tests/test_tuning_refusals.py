@@ -38,6 +38,9 @@ def test_cpu_tensors_and_shapes():
         PolicyLoss()(x[0], x[0], torch.zeros(5))
     with pytest.raises(AssertionError, match="one to a sequence"):
         PolicyLoss()(x, x, torch.zeros(3, 4))
+    for advantages in (torch.zeros(3, 1), torch.zeros(3, 1).expand(3, 0), torch.zeros(3, 0)):      # all of them are taken
+        with pytest.raises(AssertionError, match="cuda"):
+            PolicyLoss()(x[:, :0], x[:, :0], advantages)
     with pytest.raises(AssertionError, match="cuda"):
         PreferenceLoss()(torch.zeros(4, 5))
     with pytest.raises(AssertionError, match="pairs"):
