@@ -12,8 +12,6 @@ import array
 import ctypes
 import os
 
-import torch as _torch
-
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "csrc", "libbmt_hip.so")
 
@@ -124,43 +122,6 @@ def clip_table(sources, destinations, counts, source_types, destination_types):
     return array.array("q", words)
 
 
-def _tensor_reader():
-    """Address of the installed torch's dltensor_from_py_object_no_sync (the fifth entry of its DLPack exchange table,
-    behind the 16-byte header), or None where it offers no such table of version 1."""
-    capsule = getattr(_torch.Tensor, "__dlpack_c_exchange_api__", None)
-    if capsule is None:
-        return None
-    pointer_of = ctypes.pythonapi.PyCapsule_GetPointer
-    pointer_of.restype, pointer_of.argtypes = _p, [ctypes.py_object, ctypes.c_char_p]
-    table = pointer_of(capsule, b"dlpack_exchange_api")
-    if not table or ctypes.cast(table, ctypes.POINTER(ctypes.c_uint32))[0] != 1:
-        return None
-    return ctypes.cast(table, ctypes.POINTER(_p))[5]
-
-
-_read_tensor = _tensor_reader()
-_item_of = ctypes.cast(ctypes.pythonapi.PyList_GetItem, _p).value
-# called with the interpreter's lock held: it calls back into Python's own functions
-_from_tensors = ctypes.PyDLL(LIBRARY_PATH).clip_table_from_tensors
-_from_tensors.restype = ctypes.c_int
-_from_tensors.argtypes = [ctypes.py_object, ctypes.py_object, _i32, _p, _p, _p, ctypes.POINTER(_i32)]
-_tensor_types = {_torch.Tensor, _torch.nn.Parameter}
-
-
-def clip_table_from_tensors(sources: list, destinations: list):
-    """(`bmt_clip_tensor` array, device) of two lists of contiguous GPU tensors (the same list twice: in place), read by the
-    library itself; None where they are not all of that kind, or torch does not offer the means."""
-    if _read_tensor is None or not sources or type(sources) is not list or type(destinations) is not list:
-        return None
-    if len(sources) != len(destinations) or not (set(map(type, sources)) | set(map(type, destinations))) <= _tensor_types:
-        return None
-    table = array.array("q", bytes(32 * len(sources)))
-    device = _i32()
-    status = _from_tensors(sources, destinations, len(sources), _item_of, _read_tensor, table.buffer_info()[0],
-                           ctypes.byref(device))
-    return (table, device.value) if status == 0 else None
-
-
 _lib.bmt_hip_flat_stream_stats.restype = ctypes.c_int
 _lib.bmt_hip_flat_stream_stats.argtypes = [ctypes.POINTER(_i64)]
 
@@ -223,6 +184,6 @@ adam_fp16_multi_clip_launcher = _bind_multi("adam_fp16_multi_clip_launcher", 1)
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + ["is_bf16_supported", "bmt_hip_last_error", "grad_stats_workspace_floats",
                                                   "bmt_hip_flat_stream_stats", "grad_stats_multi_launcher",
                                                   "policy_loss_workspace_doubles", "preference_loss_workspace_doubles",
-                                                  "grad_norm_workspace_doubles", "clip_table_from_tensors",
+                                                  "grad_norm_workspace_doubles",
                                                   "adam_bf16_multi_launcher", "adam_fp16_multi_launcher",
                                                   "adam_bf16_multi_clip_launcher", "adam_fp16_multi_clip_launcher"])

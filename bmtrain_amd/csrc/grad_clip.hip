@@ -310,67 +310,6 @@ hipError_t scale_from(int32_t count, const bmt_clip_tensor *tensors, int32_t src
 }  // namespace
 }  // namespace bmt
 
-namespace bmt {
-namespace {
-
-// The layout in which the DLPack protocol (version 1) describes a tensor.
-struct DlTensor {
-    void *data;
-    int32_t device_type, device_id, ndim;
-    uint8_t code, bits;
-    uint16_t lanes;
-    int64_t *shape, *strides;
-    uint64_t byte_offset;
-};
-typedef int (*ReadTensor)(void *object, DlTensor *out);
-typedef void *(*ItemOf)(void *list, std::ptrdiff_t index);
-
-// Pointer, count and type code of a contiguous GPU tensor; false where it is anything else.
-bool plain_tensor(const DlTensor &t, int32_t *device, void **data, int64_t *n, int32_t *type) {
-    constexpr int32_t kCuda = 2, kRocm = 10;
-    constexpr uint8_t kFloat = 2, kBfloat = 4;
-    if ((t.device_type != kCuda && t.device_type != kRocm) || t.lanes != 1) return false;
-    if (*device < 0) *device = t.device_id;
-    if (*device != t.device_id) return false;
-    if (t.code == kFloat && t.bits == 32) *type = kFp32;
-    else if (t.code == kFloat && t.bits == 16) *type = kFp16;
-    else if (t.code == kBfloat && t.bits == 16) *type = kBf16;
-    else return false;
-    int64_t count = 1;
-    for (int32_t d = t.ndim - 1; d >= 0; d--) {
-        if (t.strides && t.shape[d] != 1 && t.strides[d] != count) return false;
-        count *= t.shape[d];
-    }
-    *data = (char *)t.data + t.byte_offset;
-    *n = count;
-    return true;
-}
-
-}  // namespace
-}  // namespace bmt
-
-extern "C" int clip_table_from_tensors(void *sources, void *destinations, int32_t count, void *item_of, void *read_tensor,
-                                       bmt_clip_tensor *table, int32_t *device) {
-    using namespace bmt;
-    if (!sources || !item_of || !read_tensor || !table || !device) return 1;
-    const ItemOf item = (ItemOf)item_of;
-    const ReadTensor read = (ReadTensor)read_tensor;
-    *device = -1;
-    for (int32_t k = 0; k < count; k++) {
-        DlTensor t;
-        bmt_clip_tensor &row = table[k];
-        void *object = item(sources, k), *data = nullptr;
-        if (!object || read(object, &t) != 0 || !plain_tensor(t, device, &data, &row.n, &row.src_type)) return 1;
-        row.src = data, row.dst = data, row.dst_type = row.src_type;
-        if (destinations && destinations != sources) {
-            int64_t n = 0;
-            object = item(destinations, k);
-            if (!object || read(object, &t) != 0 || !plain_tensor(t, device, &row.dst, &n, &row.dst_type) || n != row.n) return 1;
-        }
-    }
-    return 0;
-}
-
 extern "C" int64_t grad_norm_workspace_doubles(int32_t count, const bmt_clip_tensor *tensors) {
     int64_t tiles = 1;
     if (tensors)

@@ -1,7 +1,7 @@
 from .cross_entropy import FusedCrossEntropy, OpFusedCrossEntropy, VPFusedCrossEntropy
-from .token_logprobs import OpTokenLogProbs, TokenLogProbs
-from .policy import OpPolicyLoss, PolicyLoss
-from .preference import OpPreferenceLoss, PreferenceLoss
+from .token_logprobs import TokenLogProbs
+from .policy import PolicyLoss
+from .preference import PreferenceLoss
 
-__all__ = ["FusedCrossEntropy", "OpFusedCrossEntropy", "VPFusedCrossEntropy", "OpTokenLogProbs", "TokenLogProbs",
-           "OpPolicyLoss", "PolicyLoss", "OpPreferenceLoss", "PreferenceLoss"]
+__all__ = ["FusedCrossEntropy", "OpFusedCrossEntropy", "VPFusedCrossEntropy", "TokenLogProbs", "PolicyLoss",
+           "PreferenceLoss"]

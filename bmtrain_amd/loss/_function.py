@@ -3,8 +3,6 @@ launchers.  Same functions, argument order and exception types as
 bmtrain/loss/_function.py (ValueError for a dtype that is not 16-bit,
 NotImplementedError when bf16 is unavailable, AssertionError for the rest).
 """
-import contextlib
-
 import torch
 
 from .. import C
@@ -134,213 +132,3 @@ def loss_reduce_backward(target: torch.Tensor, weight, n_classes: int, ignore_in
                                              weight.data_ptr() if weight is not None else 0, n_classes, ignore_index,
                                              int(mean), weight_sum.data_ptr(), upstream.data_ptr(), grad_rows.data_ptr(),
                                              _current_stream())
-
-
-# ---- token log-probabilities, policy and preference losses: fp32, fp16 and bf16 alike --------------------------------
-# Small batches are bound by the host: the checks below read every property once, and scratch of one call is one
-# allocation.
-
-_TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_MASK_TYPES = (torch.bool, torch.uint8)
-
-
-def _type_code(op: str, dtype: torch.dtype) -> int:
-    code = _TYPE_CODES.get(dtype)
-    if code is None:
-        raise ValueError(f"{op} not supported for dtype {dtype}")
-    return code
-
-
-def _stream_of(device: int) -> int:
-    """The current stream of GPU `device` (what torch.cuda.current_stream wraps into an object)."""
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-_HERE = contextlib.nullcontext()
-
-
-def on_device_of(t: torch.Tensor):
-    """The context in which launches go to the device of `t`."""
-    assert t.is_cuda, "tensors must be on cuda"
-    device = t.get_device()
-    return _HERE if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
-
-
-def _ptr(t) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _dense(name: str, t, device: int, dtype: torch.dtype, numel: int) -> int:
-    """Pointer of a contiguous tensor of `numel` elements on `device`; 0 for None."""
-    if t is None:
-        return 0
-    assert t.get_device() == device, f"{name} must be on the same cuda device as the other tensors"
-    assert t.is_contiguous() and t.dtype == dtype and t.numel() == numel, f"{name} must be {numel} contiguous elements of {dtype}"
-    return t.data_ptr()
-
-
-def row_layout(logits: torch.Tensor):
-    """(logits, rows, n, inner, outer stride, inner stride) of logits [..., n]: at most two strides lead from row to row
-    and the classes lie next to each other; a tensor laid out otherwise is copied first."""
-    dims, shape, strides = logits.dim(), logits.shape, logits.stride()
-    n = shape[-1]
-    if dims > 3 or (n > 1 and strides[-1] != 1):
-        logits = logits.contiguous()
-        rows = logits.numel() // n if n else 0
-        return logits, rows, n, max(rows, 1), 0, n
-    if dims == 1:
-        return logits, 1, n, 1, 0, n
-    if dims == 2:
-        return logits, shape[0], n, max(shape[0], 1), 0, strides[0]
-    return logits, shape[0] * shape[1], n, max(shape[1], 1), strides[0], strides[1]
-
-
-def _targets(target: torch.Tensor, device: int, rows: int):
-    """Pointer and bits of the targets."""
-    assert target.get_device() == device, "target must be on the same cuda device as the logits"
-    assert target.dtype in (torch.int32, torch.int64), "target must be an int or long tensor"
-    assert target.is_contiguous() and target.numel() == rows, "target must be contiguous, one class to a row of the logits"
-    return target.data_ptr(), 32 if target.dtype == torch.int32 else 64
-
-
-def token_logprobs_forward(layout, target: torch.Tensor, ignore_index: int, temperature: float, logprob: torch.Tensor,
-                           entropy, stats) -> None:
-    """``logprob`` (and ``entropy``, or None) of the tokens ``target`` under the logits of ``layout`` (``row_layout``);
-    ``stats`` (fp32, 4 per row, or None) keeps what ``token_logprobs_backward`` needs."""
-    logits, rows, n, inner, outer_stride, inner_stride = layout
-    assert logits.is_cuda, "logits must be on cuda"
-    device = logits.get_device()
-    code = _type_code("token_logprobs", logits.dtype)
-    assert n > 0 or rows == 0, "logits must have at least one class"
-    C.token_logprobs_forward_launcher(rows, n, inner, outer_stride, inner_stride, logits.data_ptr(), code,
-                                      *_targets(target, device, rows), ignore_index, temperature,
-                                      _dense("logprob", logprob, device, torch.float32, rows),
-                                      _dense("entropy", entropy, device, torch.float32, rows),
-                                      _dense("stats", stats, device, torch.float32, 4 * rows), _stream_of(device))
-
-
-def token_logprobs_backward(layout, target: torch.Tensor, ignore_index: int, temperature: float, stats: torch.Tensor,
-                            grad_logprob, grad_entropy, grad: torch.Tensor) -> None:
-    """``grad`` (contiguous, the logits' shape and type) from the gradients of the log-probabilities and entropies
-    (contiguous fp32, either may be None)."""
-    logits, rows, n, inner, outer_stride, inner_stride = layout
-    assert logits.is_cuda, "logits must be on cuda"
-    device = logits.get_device()
-    C.token_logprobs_backward_launcher(rows, n, inner, outer_stride, inner_stride, logits.data_ptr(),
-                                       _type_code("token_logprobs", logits.dtype), *_targets(target, device, rows), ignore_index,
-                                       temperature, _dense("stats", stats, device, torch.float32, 4 * rows),
-                                       _dense("grad_logprob", grad_logprob, device, torch.float32, rows),
-                                       _dense("grad_entropy", grad_entropy, device, torch.float32, rows),
-                                       _dense("grad", grad, device, logits.dtype, rows * n), _stream_of(device))
-
-
-def _tokens(name: str, t, shape, dtype, device: int):
-    """Pointer and row stride of a [rows, time] tensor whose tokens lie next to each other; (0, 0) for None."""
-    if t is None:
-        return 0, 0
-    assert t.get_device() == device, f"{name} must be on the same cuda device as the other tensors"
-    assert t.shape == shape, f"{name} must have the shape of logprob"
-    row, token = t.stride()
-    assert token == 1 or shape[1] <= 1, f"{name}'s tokens must lie next to each other"
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must have the dtype of logprob, {dtype}")
-    return t.data_ptr(), row
-
-
-def _mask(mask, shape, device: int):
-    if mask is None:
-        return 0, 0                                     # every token counts
-    assert mask.dtype in _MASK_TYPES, "mask must be a bool or uint8 tensor"
-    return _tokens("mask", mask, shape, mask.dtype, device)
-
-
-def policy_loss_scratch(rows: int, time: int, by_row: bool, keep: bool):
-    """(floats, offset of the weights, offset of the saved derivatives or -1) of the scratch ``policy_loss_forward``
-    and ``policy_loss_backward`` share: the workspace's doubles, the weights, the derivative of every token."""
-    weights = 2 * C.policy_loss_workspace_doubles(rows, time)
-    saved = weights + (1 + rows if by_row else 1)
-    saved += -saved % 4
-    return (saved + rows * time, weights, saved) if keep else (saved, weights, -1)
-
-
-def policy_loss_forward(logprob, old_logprob, ref_logprob, entropy, advantages, mask, clip_low: float, clip_high: float,
-                        dual_clip: float, kl_coef: float, entropy_coef: float, reduction: int, scratch, offsets, loss,
-                        stats) -> None:
-    """Loss and statistics of include/bmt_hip.h ``policy_loss_forward_launcher`` for [rows, time] tensors;
-    ``advantages`` is fp32, [rows] or [rows, time]; ``mask`` bool / uint8 or None; ``scratch`` and ``offsets`` as
-    ``policy_loss_scratch`` says."""
-    assert logprob.is_cuda, "tensors must be on cuda"
-    assert logprob.dim() == 2, "logprob must be [sequences, tokens]"
-    device, shape, dtype = logprob.get_device(), logprob.shape, logprob.dtype
-    code = _type_code("policy_loss", dtype)
-    rows, time = shape
-    assert advantages.dtype == torch.float32, "advantages must be a float tensor"
-    if advantages.dim() == 2:
-        advantage, advantage_row = _tokens("advantages", advantages, shape, torch.float32, device)
-        per_token = 1
-    else:
-        assert advantages.shape == (rows,), "advantages must be one to a sequence or one to a token"
-        assert advantages.get_device() == device, "advantages must be on the same cuda device as the other tensors"
-        advantage, advantage_row, per_token = advantages.data_ptr(), advantages.stride(0), 0
-    floats, weights, saved = offsets
-    assert scratch.numel() == floats, "scratch must be what policy_loss_scratch says"
-    base = scratch.data_ptr()
-    C.policy_loss_forward_launcher(rows, time, code, *_tokens("logprob", logprob, shape, dtype, device),
-                                   *_tokens("old_logprob", old_logprob, shape, dtype, device),
-                                   *_tokens("ref_logprob", ref_logprob, shape, dtype, device),
-                                   *_tokens("entropy", entropy, shape, dtype, device), advantage, advantage_row, per_token,
-                                   *_mask(mask, shape, device), clip_low, clip_high, dual_clip, kl_coef, entropy_coef, reduction,
-                                   base + 4 * saved if saved >= 0 else 0, base + 4 * weights, base, loss.data_ptr(),
-                                   stats.data_ptr(), _stream_of(device))
-
-
-def policy_loss_backward(reduction: int, scratch, offsets, upstream, mask, entropy_coef: float, grad_logprob, grad_entropy) -> None:
-    """Gradients (contiguous [rows, time], of the log-probabilities' type; either may be None) of ``policy_loss_forward``."""
-    first = grad_logprob if grad_logprob is not None else grad_entropy
-    if first is None:
-        return
-    device, shape = first.get_device(), first.shape
-    floats, weights, saved = offsets
-    assert scratch.numel() == floats and (saved >= 0 or grad_logprob is None), "scratch must be that of the forward call"
-    assert upstream.get_device() == device and upstream.dtype == torch.float32 and upstream.numel() == 1, "upstream must be one float on cuda"
-    base = scratch.data_ptr()
-    C.policy_loss_backward_launcher(*shape, _TYPE_CODES[first.dtype], reduction, base + 4 * saved if saved >= 0 else 0,
-                                    base + 4 * weights, upstream.data_ptr(), *((0, 0) if mask is None else (mask.data_ptr(), mask.stride(0))),
-                                    entropy_coef, _ptr(grad_logprob), _ptr(grad_entropy), _stream_of(device))
-
-
-def preference_loss_scratch(pairs: int, time: int):
-    """(floats, offset of the slopes) of the scratch ``preference_loss_forward`` and ``preference_loss_backward`` share:
-    the workspace's doubles, then one slope per row behind their common factor."""
-    slope = 2 * C.preference_loss_workspace_doubles(pairs, time)
-    return slope + 1 + 2 * pairs, slope
-
-
-def preference_loss_forward(logprob, ref_logprob, mask, kind: int, average: bool, beta: float, label_smoothing: float, scratch,
-                            offsets, loss, chosen, rejected) -> None:
-    """Loss and rewards of include/bmt_hip.h ``preference_loss_forward_launcher`` for [2 * pairs, time] tensors, the
-    chosen answers in front of the rejected ones; ``scratch`` and ``offsets`` as ``preference_loss_scratch`` says."""
-    assert logprob.is_cuda, "tensors must be on cuda"
-    assert logprob.dim() == 2 and logprob.size(0) % 2 == 0, "logprob must be [2 * pairs, tokens]"
-    device, shape, dtype = logprob.get_device(), logprob.shape, logprob.dtype
-    code = _type_code("preference_loss", dtype)
-    pairs = shape[0] // 2
-    floats, slope = offsets
-    assert scratch.numel() == floats, "scratch must be what preference_loss_scratch says"
-    base = scratch.data_ptr()
-    C.preference_loss_forward_launcher(pairs, shape[1], code, *_tokens("logprob", logprob, shape, dtype, device),
-                                       *_tokens("ref_logprob", ref_logprob, shape, dtype, device), *_mask(mask, shape, device),
-                                       kind, int(average), beta, label_smoothing, base, loss.data_ptr(), chosen.data_ptr(),
-                                       rejected.data_ptr(), base + 4 * slope, _stream_of(device))
-
-
-def preference_loss_backward(scratch, offsets, upstream, mask, grad_logprob) -> None:
-    """Gradient (contiguous [2 * pairs, time]) of ``preference_loss_forward``."""
-    rows, time = grad_logprob.shape
-    floats, slope = offsets
-    assert scratch.numel() == floats, "scratch must be that of the forward call"
-    device = grad_logprob.get_device()
-    assert upstream.get_device() == device and upstream.dtype == torch.float32 and upstream.numel() == 1, "upstream must be one float on cuda"
-    C.preference_loss_backward_launcher(rows // 2, time, _TYPE_CODES[grad_logprob.dtype], scratch.data_ptr() + 4 * slope,
-                                        upstream.data_ptr(), *((0, 0) if mask is None else (mask.data_ptr(), mask.stride(0))),
-                                        grad_logprob.data_ptr(), _stream_of(device))

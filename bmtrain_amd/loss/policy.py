@@ -3,63 +3,10 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .. import C
-from . import _function as F
+from .. import _tensors
 
 _REDUCTIONS = {"mean": 0, "sequence": 1, "sum": 2}
-
-
-def _tokens_adjacent(t):
-    """`t` with its last dimension's elements next to each other (a copy where they are not); None stays None."""
-    return t if t is None or t.is_contiguous() or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def constant(t):
-    """`t` without its gradient, its tokens next to each other; None stays None."""
-    return _tokens_adjacent(t.detach() if t is not None and t.requires_grad else t)
-
-
-def as_mask(mask):
-    """A bool / uint8 mask as it is; anything else as ``mask != 0``."""
-    if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
-        mask = mask != 0
-    return _tokens_adjacent(mask)
-
-
-class OpPolicyLoss(torch.autograd.Function):
-    """Loss and statistics in two launches, both gradients in one."""
-
-    @staticmethod
-    def forward(ctx, logprob, entropy, old_logprob, advantages, mask, ref_logprob, clips, kl_coef, entropy_coef, reduction):
-        with F.on_device_of(logprob):
-            shape, device = logprob.shape, logprob.device
-            offsets = F.policy_loss_scratch(*shape, reduction == 1, ctx.needs_input_grad[0])
-            loss = torch.empty((), device=device, dtype=torch.float)
-            stats = torch.empty(5, device=device, dtype=torch.float)
-            scratch = torch.empty(offsets[0], device=device, dtype=torch.float)
-            F.policy_loss_forward(logprob, old_logprob, ref_logprob, entropy, advantages, mask, *clips, kl_coef, entropy_coef,
-                                  reduction, scratch, offsets, loss, stats)
-        ctx.args = (reduction, offsets, entropy_coef, shape, logprob.dtype)
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)                # nothing is to be filled with zeros for the statistics
-        ctx.save_for_backward(scratch, mask)
-        return loss, stats
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, upstream, _):
-        if upstream is None:
-            return (None,) * 10
-        scratch, mask = ctx.saved_tensors
-        reduction, offsets, entropy_coef, shape, dtype = ctx.args
-        with F.on_device_of(scratch):
-            device = scratch.device
-            grad_logprob = torch.empty(shape, device=device, dtype=dtype) if ctx.needs_input_grad[0] else None
-            grad_entropy = torch.empty(shape, device=device, dtype=dtype) if ctx.needs_input_grad[1] else None
-            F.policy_loss_backward(reduction, scratch, offsets, upstream, mask, entropy_coef, grad_logprob, grad_entropy)
-        return grad_logprob, grad_entropy, None, None, None, None, None, None, None, None
 
 
 class PolicyLoss(torch.nn.Module):
@@ -108,14 +55,5 @@ class PolicyLoss(torch.nn.Module):
     def forward(self, logprob: torch.Tensor, old_logprob: torch.Tensor, advantages: torch.Tensor,
                 mask: Optional[torch.Tensor] = None, ref_logprob: Optional[torch.Tensor] = None,
                 entropy: Optional[torch.Tensor] = None):
-        assert logprob.dim() == 2, "logprob must be [sequences, tokens]"
-        if advantages.dim() == 2 and advantages.size(1) and (advantages.shape != logprob.shape or advantages.stride(1) == 0):
-            assert advantages.size(1) == 1 or advantages.shape == logprob.shape, "advantages must be one to a sequence or one to a token"
-            advantages = advantages[:, 0]              # one to a sequence: [sequences, 1], or an expanded view
-        if advantages.dtype != torch.float32:
-            advantages = advantages.float()
-        advantages = constant(advantages) if advantages.dim() == 2 else advantages.detach() if advantages.requires_grad else advantages
-        return OpPolicyLoss.apply(_tokens_adjacent(logprob), _tokens_adjacent(entropy), constant(old_logprob), advantages,
-                                  as_mask(mask), constant(ref_logprob),
-                                  (self.clip_low, self.clip_high, self.dual_clip or 0.0), self.kl_coef, self.entropy_coef,
-                                  _REDUCTIONS[self.reduction])
+        return _tensors.policy_loss(logprob, old_logprob, advantages, mask, ref_logprob, entropy, self.clip_low, self.clip_high,
+                                    self.dual_clip or 0.0, self.kl_coef, self.entropy_coef, _REDUCTIONS[self.reduction])

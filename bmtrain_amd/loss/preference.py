@@ -3,47 +3,10 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .. import C
-from . import _function as F
-from .policy import _tokens_adjacent, as_mask, constant
+from .. import _tensors
 
 _KINDS = {"sigmoid": 0, "ipo": 1, "hinge": 2}
-
-
-class OpPreferenceLoss(torch.autograd.Function):
-    """Loss and both rewards in two launches, the gradient in one."""
-
-    @staticmethod
-    def forward(ctx, logprob, ref_logprob, mask, kind, average, beta, label_smoothing):
-        with F.on_device_of(logprob):
-            shape, device = logprob.shape, logprob.device
-            pairs = shape[0] // 2
-            offsets = F.preference_loss_scratch(pairs, shape[1])
-            loss = torch.empty((), device=device, dtype=torch.float)
-            chosen = torch.empty(pairs, device=device, dtype=torch.float)
-            rejected = torch.empty(pairs, device=device, dtype=torch.float)
-            scratch = torch.empty(offsets[0], device=device, dtype=torch.float)
-            F.preference_loss_forward(logprob, ref_logprob, mask, kind, average, beta, label_smoothing, scratch, offsets, loss,
-                                      chosen, rejected)
-        ctx.args = (offsets, shape, logprob.dtype)
-        ctx.mark_non_differentiable(chosen, rejected)
-        ctx.set_materialize_grads(False)                # nothing is to be filled with zeros for the rewards
-        ctx.save_for_backward(scratch, mask)
-        return loss, chosen, rejected
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, upstream, *_):
-        if upstream is None:
-            return (None,) * 7
-        scratch, mask = ctx.saved_tensors
-        offsets, shape, dtype = ctx.args
-        with F.on_device_of(scratch):
-            grad = torch.empty(shape, device=scratch.device, dtype=dtype)
-            F.preference_loss_backward(scratch, offsets, upstream, mask, grad)
-        return grad, None, None, None, None, None, None
 
 
 class PreferenceLoss(torch.nn.Module):
@@ -78,8 +41,5 @@ class PreferenceLoss(torch.nn.Module):
         self.beta, self.kind, self.label_smoothing, self.average = float(beta), kind, float(label_smoothing), average
 
     def forward(self, logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
-        if logprob.dim() == 1:
-            logprob, ref_logprob, mask = [t if t is None else t.unsqueeze(1) for t in (logprob, ref_logprob, mask)]
-        assert logprob.dim() == 2 and logprob.size(0) % 2 == 0, "logprob must be [2 * pairs, tokens]"
-        return OpPreferenceLoss.apply(_tokens_adjacent(logprob), constant(ref_logprob), as_mask(mask), _KINDS[self.kind], bool(self.average),
-                                      self.beta, self.label_smoothing)
+        return _tensors.preference_loss(logprob, ref_logprob, mask, _KINDS[self.kind], bool(self.average), self.beta,
+                                        self.label_smoothing)

@@ -6,48 +6,8 @@ log-probability of every token as a value with a gradient, often under a tempera
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _function as F
-
-
-def _forward(logits, target, ignore_index, temperature, entropy, keep):
-    """(logprob or (logprob, entropy), what the backward pass needs if `keep`)."""
-    with F.on_device_of(logits):
-        layout = F.row_layout(logits)
-        device = logits.device
-        logprob = torch.empty(target.shape, device=device, dtype=torch.float)
-        entropies = torch.empty(target.shape, device=device, dtype=torch.float) if entropy else None
-        stats = torch.empty((layout[1], 4), device=device, dtype=torch.float) if keep else None
-        F.token_logprobs_forward(layout, target, ignore_index, temperature, logprob, entropies, stats)
-    return ((logprob, entropies) if entropy else logprob), stats
-
-
-class OpTokenLogProbs(torch.autograd.Function):
-    """fp32 ``log softmax(logits / temperature)[target]`` per token (and the entropy of every token's distribution).
-    Keeps the logits and four numbers per token for the backward pass, which reads the logits once more."""
-
-    @staticmethod
-    def forward(ctx, logits: torch.Tensor, target: torch.Tensor, ignore_index: int, temperature: float, entropy: bool):
-        target = target.contiguous()
-        out, stats = _forward(logits, target, ignore_index, temperature, entropy, ctx.needs_input_grad[0])
-        ctx.args = (ignore_index, temperature)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, target, stats)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_logprob, grad_entropy=None):
-        if grad_logprob is None and grad_entropy is None:
-            return None, None, None, None, None
-        logits, target, stats = ctx.saved_tensors
-        with F.on_device_of(logits):
-            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-            F.token_logprobs_backward(F.row_layout(logits), target, *ctx.args, stats,
-                                      None if grad_logprob is None else grad_logprob.contiguous(),
-                                      None if grad_entropy is None else grad_entropy.contiguous(), grad)
-        return grad, None, None, None, None
+from .. import _tensors
 
 
 class TokenLogProbs(torch.nn.Module):
@@ -85,7 +45,5 @@ class TokenLogProbs(torch.nn.Module):
         self.entropy = entropy
 
     def forward(self, logits: torch.Tensor, target: torch.Tensor):
-        assert logits.dim() >= 1 and logits.shape[:-1] == target.shape, "target must have the shape of logits without its last dimension"
-        if not (logits.requires_grad and torch.is_grad_enabled()):          # scoring: nothing to remember
-            return _forward(logits, target.contiguous(), self.ignore_index, self.temperature, self.entropy, False)[0]
-        return OpTokenLogProbs.apply(logits, target, self.ignore_index, self.temperature, self.entropy)
+        logprob, entropy = _tensors.token_logprobs(logits, target, self.ignore_index, self.temperature, self.entropy)
+        return (logprob, entropy) if self.entropy else logprob

@@ -205,76 +205,3 @@ def adam_multi(tensors, beta1: float, beta2: float, eps: float, lr: float, scale
         launcher = C.adam_bf16_multi_clip_launcher if flavour == torch.bfloat16 else C.adam_fp16_multi_clip_launcher
         launcher(rows, beta1, beta2, eps, lr, scale, weight_decay, bias_correction1, bias_correction2, grad_coef,
                  _current_stream())
-
-
-_TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_Tensor = torch.Tensor
-
-
-def _codes(tensors):
-    dtypes = [t.dtype for t in tensors]
-    kinds = set(dtypes)
-    for dtype in kinds:
-        if dtype not in _TYPE_CODES:
-            raise ValueError(f"gradients must be fp32, fp16 or bf16, not {dtype}")
-    return [_TYPE_CODES[dtypes[0]]] * len(dtypes) if len(kinds) == 1 else [_TYPE_CODES[dtype] for dtype in dtypes]
-
-
-def clip_table(grads, outs=None):
-    """``C.clip_table`` of dense GPU tensors of fp32, fp16 or bf16 on one device; ``outs`` (default: the gradients
-    themselves) have their gradients' numbers of elements, and their strides where a gradient is not contiguous.  With
-    many small gradients this is what a call costs: lists of contiguous tensors are read by the library, anything else
-    (and what is to be refused) here, every property once for the whole list."""
-    outs = grads if outs is None else outs
-    read = C.clip_table_from_tensors(grads, outs)
-    if read is not None:
-        return read[0]
-    codes = _codes(grads)
-    sources = list(map(_Tensor.data_ptr, grads))
-    counts = list(map(_Tensor.numel, grads))
-    devices = set(map(_Tensor.get_device, grads))
-    dense = all(map(_Tensor.is_contiguous, grads))
-    if outs is grads:
-        out_codes, destinations = codes, sources
-        assert dense or all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
-    else:
-        out_codes = _codes(outs)
-        destinations = list(map(_Tensor.data_ptr, outs))
-        devices.update(map(_Tensor.get_device, outs))
-        assert counts == list(map(_Tensor.numel, outs)), "outputs must have their gradients' numbers of elements"
-        if not (dense and all(map(_Tensor.is_contiguous, outs))):
-            assert all(map(is_dense, grads)), "gradients must not have gaps nor elements that share memory"
-            assert all((g.is_contiguous() and o.is_contiguous()) or (g.shape == o.shape and g.stride() == o.stride())
-                       for g, o in zip(grads, outs)), "outputs must have their gradients' strides"
-    assert len(devices) == 1 and -1 not in devices, "gradients must be on one cuda device"
-    return C.clip_table(sources, destinations, counts, codes, out_codes)
-
-
-def is_dense(t: torch.Tensor) -> bool:
-    """True if the elements of `t` fill one run of memory without gaps, in whatever order of dimensions."""
-    expected = 1
-    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
-        if stride != expected:
-            return t.numel() == 0
-        expected *= size
-    return True
-
-
-def grad_norm_multi(table, use_max: bool, max_norm: float, eps: float, scale: float, out: torch.Tensor) -> None:
-    """``out[0] = n / scale`` and the clipping factor ``out[1] = max_norm * scale / (n + eps)`` for n the L2 norm (or the
-    largest magnitude) over the gradients of ``table`` (``clip_table``); ``out`` is two floats."""
-    assert out.is_cuda and out.dtype == torch.float32 and out.numel() == 2 and out.is_contiguous()
-    address, words = table.buffer_info()
-    device = out.get_device()
-    workspace = torch.empty(C.grad_norm_workspace_doubles(words // 4, address), dtype=torch.float64, device=out.device)
-    C.grad_norm_multi_launcher(words // 4, address, int(use_max), max_norm, eps, scale, workspace.data_ptr(), out.data_ptr(),
-                               torch._C._cuda_getCurrentRawStream(device))
-
-
-def grad_scale_multi(table, coef: torch.Tensor, round_coef: bool = False) -> None:
-    """Every destination of ``table`` = its source times ``coef`` (one float on the GPU) if that is below one, else the
-    source itself; ``round_coef``: times the factor rounded to the source's type."""
-    assert coef.is_cuda and coef.dtype == torch.float32 and coef.numel() == 1, "coef must be one float on cuda"
-    address, words = table.buffer_info()
-    C.grad_scale_multi_launcher(words // 4, address, coef.data_ptr(), int(round_coef),
-                                torch._C._cuda_getCurrentRawStream(coef.get_device()))

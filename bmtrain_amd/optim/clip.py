@@ -6,12 +6,9 @@ from typing import Optional, Sequence
 
 import torch
 
-from ..loss._function import on_device_of
-from . import _function as F
+from .. import _tensors
 
 
-
-@torch.no_grad()
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, eps: float = 1e-6, scale: float = 1.0,
                out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     r"""Clips ``grads`` to the global norm ``max_norm`` and returns their norm before clipping, a 0-dim fp32 tensor on
@@ -54,13 +51,4 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         raise ValueError(f"norm_type must be 2 or inf, not {norm_type}")
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda" if torch.cuda.is_available() else "cpu")
-    table = F.clip_table(grads, outs)
-    with on_device_of(grads[0]):
-        result = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-        F.grad_norm_multi(table, use_max, float(max_norm), float(eps), float(scale), result)
-        F.grad_scale_multi(table, result[1])
-    try:
-        torch.autograd.graph.increment_version(outs)        # autograd is to notice the write, as with any in-place operation
-    except RuntimeError:                                    # inference tensors: nothing keeps them for a backward pass
-        pass
-    return result[0]
+    return _tensors.clip_grads(grads, None if out is None else outs, float(max_norm), use_max, float(eps), float(scale))

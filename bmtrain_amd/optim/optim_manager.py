@@ -9,10 +9,11 @@ from typing import Optional
 
 import torch
 
+from .. import _tensors
 from ..global_var import config
-from ..loss._function import has_inf_nan, on_device_of
+from ..loss._function import has_inf_nan
 from ._base import flat_runs
-from ._function import clip_table, grad_scale_multi, grad_stats, grad_stats_multi
+from ._function import grad_stats, grad_stats_multi
 
 
 def _scanned_grads(param_groups):
@@ -232,8 +233,7 @@ class OptimManager:
             else:
                 rest.append(g)
         if fused:
-            with on_device_of(fused[0]):
-                grad_scale_multi(clip_table(fused), clip_coef, round_coef=True)
+            _tensors.scale_grads(fused, clip_coef)
         if rest and clip_coef < 1:
             as_number = {}                  # on the GPU a Python number takes torch's vectorised scalar kernel: same bits
             for g in rest:

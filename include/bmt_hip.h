@@ -357,16 +357,6 @@ typedef struct bmt_clip_tensor {
     int64_t n;
     int32_t src_type, dst_type;
 } bmt_clip_tensor;
-/*
- * clip_table_from_tensors fills `table` from two Python lists of `count` tensors (destinations may be NULL: in place)
- * without a Python call per tensor: `item_of` is PyList_GetItem, `read_tensor` the framework's
- * dltensor_from_py_object_no_sync of the DLPack exchange table (version 1).  The caller holds the interpreter's lock and
- * has made sure of the objects' types.  Returns 0 and the tensors' device if all are contiguous fp32 / fp16 / bf16
- * tensors on one GPU and the destinations have their sources' numbers of elements, otherwise 1 (no error text; a Python
- * exception may be set): look at them one by one then.
- */
-BMT_API int clip_table_from_tensors(void *sources, void *destinations, int32_t count, void *item_of, void *read_tensor,
-                                    bmt_clip_tensor *table, int32_t *device);
 BMT_API int64_t grad_norm_workspace_doubles(int32_t count, const bmt_clip_tensor *tensors);
 BMT_API int grad_norm_multi_launcher(int32_t count, const bmt_clip_tensor *tensors, int32_t use_max, double max_norm, double eps,
                                      double scale, void *workspace, void *out, void *stream);

@@ -8,8 +8,8 @@ import math
 import pytest
 import torch
 
-from bmtrain_amd import C
-from bmtrain_amd.optim import OptimManager, clip_grads, _function as OF
+from bmtrain_amd import _tensors
+from bmtrain_amd.optim import OptimManager, clip_grads
 
 pytestmark = pytest.mark.gpu
 
@@ -223,22 +223,18 @@ def test_manager_scales_with_the_same_bits(dtypes):
         assert torch.equal(twice.grad, b.mul_(coef).mul_(coef) if coef < 1 else b)
 
 
-def test_both_ways_of_reading_tensors_agree(monkeypatch):
-    """The table the library reads by itself against the one built property by property; lists it does not take."""
+def test_tensors_of_every_kind_in_one_list():
+    """Views, parameters, leaves, scalars, empty tensors and transposed columns next to each other."""
     base = torch.randn(7, 11, device="cuda")
-    grads = [base, base[2:5], torch.empty(0, 3, device="cuda"), torch.nn.Parameter(torch.zeros(5, device="cuda")), torch.zeros((), device="cuda"),
-             torch.zeros(6, device="cuda", requires_grad=True), base[1:2, :].t(), base.bfloat16()[:, :], torch.zeros(9, device="cuda").half()]
+    grads = [base.clone(), base[2:5], torch.empty(0, 3, device="cuda"), torch.nn.Parameter(torch.ones(5, device="cuda")), torch.ones((), device="cuda"),
+             torch.ones(6, device="cuda", requires_grad=True), base.clone()[1:2, :].t(), base.bfloat16()[:, :], torch.ones(9, device="cuda").half()]
     outs = [torch.empty_like(g, dtype=torch.bfloat16) for g in grads]
-    read = C.clip_table_from_tensors(grads, outs)
-    if read is None:
-        pytest.skip("this torch offers no DLPack exchange table")
-    read_in_place = C.clip_table_from_tensors(grads, grads)
-    for bad in ([base.t()], [base[:, 1:]], [base.double()], [base.cpu()], [base.int()], [base.to(torch.complex64)]):
-        assert C.clip_table_from_tensors(bad, bad) is None
-    assert C.clip_table_from_tensors([base], [base[1:]]) is None
-    monkeypatch.setattr(C, "_read_tensor", None)
-    assert C.clip_table_from_tensors(grads, outs) is None
-    assert read == (OF.clip_table(grads, outs), 0) and read_in_place == (OF.clip_table(grads), 0)
+    with torch.no_grad():
+        check(grads, 0.3, out=outs)
+        check(grads, 0.3)
+    for bad in (base[:, 1:], base.cpu(), base.int(), base.to(torch.complex64)):
+        with pytest.raises((AssertionError, ValueError)):
+            clip_grads([base, bad], 0.3)
     check([base.clone(), base.bfloat16()], 0.3, out=[torch.empty_like(base), torch.empty_like(base).half()])
 
 
@@ -269,9 +265,9 @@ def test_a_larger_grid_than_one_batch_of_every_type():
 
 
 def test_rounded_factor():
-    """grad_scale_multi with round_coef: the factor is rounded to each source's type first."""
+    """scale_grads: the factor is rounded to each gradient's type first."""
     coef = torch.tensor(0.123456, device="cuda")
     grads = grads_of([1001, 999, 1003], (torch.float32, torch.bfloat16, torch.float16), 6)
     want = [(g.float() * coef.to(g.dtype).float()).to(g.dtype) for g in grads]
-    OF.grad_scale_multi(OF.clip_table(grads), coef, round_coef=True)
+    _tensors.scale_grads(grads, coef)
     assert all(torch.equal(a, b) for a, b in zip(grads, want))

@@ -9,7 +9,8 @@ off by its probability's error times what multiplies it, plus half a step of its
 import pytest
 import torch
 
-from bmtrain_amd.loss import TokenLogProbs, _function as F
+from bmtrain_amd import _tensors
+from bmtrain_amd.loss import TokenLogProbs
 
 pytestmark = pytest.mark.gpu
 
@@ -102,7 +103,7 @@ def test_views_are_not_copied_and_give_the_same(dtype, n):
     full = (torch.randn(3, 9, n + 6, generator=gen, device="cuda") * 2).to(dtype)
     for view in (full[:, :-1, :n], full[:, 1:, 5:], full.transpose(0, 1)[:, :, 1:n], full[::2, ::3, :n], full[:, :1, :n],
                  full[1, 2, :n].expand(4, 5, n), full[0, :, :n]):
-        assert F.row_layout(view)[0].data_ptr() == view.data_ptr()
+        assert _tensors.row_layout(view)[0].data_ptr() == view.data_ptr()
         target = torch.randint(0, view.size(-1), view.shape[:-1], generator=gen, device="cuda")
         g, h = torch.randn(target.shape, generator=gen, device="cuda"), torch.randn(target.shape, generator=gen, device="cuda")
         check(view, target, g=g, h=h, temperature=1.3)

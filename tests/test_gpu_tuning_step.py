@@ -149,3 +149,78 @@ def test_two_streams_at_once():
     for k in range(2):
         for loss, grad in got[k]:
             assert torch.equal(loss, want[k][0]) and torch.equal(grad, want[k][1])
+
+
+def calls():
+    """(name, call of one leaf, the leaf, what else is kept for the backward pass)"""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    logits = torch.randn(6, 9, 50, generator=gen, device="cuda")
+    target = torch.randint(0, 50, (6, 9), generator=gen, device="cuda")
+    old, ref = -torch.rand(6, 9, generator=gen, device="cuda"), -torch.rand(6, 9, generator=gen, device="cuda")
+    mask = torch.rand(6, 9, generator=gen, device="cuda") < 0.7
+    advantages = torch.randn(6, generator=gen, device="cuda")
+    logprobs, policy, preference = bmt.loss.TokenLogProbs(entropy=True), bmt.loss.PolicyLoss(kl_coef=0.1), bmt.loss.PreferenceLoss()
+
+    def of_logits(x):
+        logprob, entropy = logprobs(x, target)
+        return (logprob * old).sum() + (entropy * ref).sum()
+    return [("logprobs", of_logits, logits, target), ("policy", lambda x: policy(x, old, advantages, mask, ref)[0], old + 0.1, mask),
+            ("preference", lambda x: preference(x, ref, mask)[0], old - 0.1, mask)]
+
+
+def test_graphs_as_autograd_knows_them():
+    """Saved-tensor hooks, recomputation, two backward passes, a second one too many, and changes to what is kept."""
+    for name, call, leaf, kept in calls():
+        x = leaf.clone().requires_grad_()
+        want, = torch.autograd.grad(call(x), x)
+        packed = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t.shape) or t.cpu(), lambda t: t.cuda()):
+            got, = torch.autograd.grad(call(x), x)
+        assert torch.equal(got, want) and len(packed) >= 2, name
+        got, = torch.autograd.grad(torch.utils.checkpoint.checkpoint(call, x, use_reentrant=False), x)
+        assert torch.equal(got, want), name
+        value = call(x)
+        first, = torch.autograd.grad(value, x, retain_graph=True)
+        second, = torch.autograd.grad(value, x)
+        assert torch.equal(first, want) and torch.equal(second, want), name
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(value, x)
+        value = call(x)
+        kept.add_(0) if kept.dtype != torch.bool else kept.logical_or_(kept)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(value, x)
+        grad, = torch.autograd.grad(call(x), x, torch.ones((), device="cuda", requires_grad=True), create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            grad.sum().backward()
+        assert call(x.detach()).grad_fn is None
+        with torch.no_grad():
+            assert call(x).grad_fn is None
+        with torch.inference_mode():
+            call(leaf.clone())
+
+
+def test_transforms_are_refused():
+    for name, call, leaf, _ in calls():
+        with pytest.raises(RuntimeError):
+            torch.func.grad(call)(leaf)
+
+
+def test_two_threads_and_streams():
+    """Calls of two threads, each on its own stream, give what one thread gives."""
+    import threading
+    want = [torch.autograd.grad(call(x), x)[0] for x, call in ((leaf.clone().requires_grad_(), call) for _, call, leaf, _ in calls())]
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            mine = calls()
+            for _ in range(30):
+                xs = [leaf.clone().requires_grad_() for _, _, leaf, _ in mine]
+                got[k] = [torch.autograd.grad(call(x), x)[0] for x, (_, call, _, _) in zip(xs, mine)]
+        torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for k in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want))

@@ -5,9 +5,9 @@ import math
 import pytest
 import torch
 
-from bmtrain_amd import C
-from bmtrain_amd.loss import PolicyLoss, PreferenceLoss, TokenLogProbs, _function as F
-from bmtrain_amd.optim import clip_grads, _function as OF
+from bmtrain_amd import C, _tensors
+from bmtrain_amd.loss import PolicyLoss, PreferenceLoss, TokenLogProbs
+from bmtrain_amd.optim import clip_grads
 
 
 def test_module_arguments():
@@ -61,41 +61,41 @@ def test_cpu_tensors_and_shapes():
 
 def test_row_layout():
     x = torch.zeros(4, 7, 10)
-    assert F.row_layout(x)[1:] == (28, 10, 7, 70, 10)
-    assert F.row_layout(x[:, :-1])[1:] == (24, 10, 6, 70, 10)
-    assert F.row_layout(x[:, :, 2:9])[1:] == (28, 7, 7, 70, 10)
-    assert F.row_layout(x[1])[1:] == (7, 10, 7, 0, 10)
-    assert F.row_layout(x[1, 2])[1:] == (1, 10, 1, 0, 10)
-    turned = F.row_layout(x.transpose(1, 2))
+    assert _tensors.row_layout(x)[1:] == (28, 10, 7, 70, 10)
+    assert _tensors.row_layout(x[:, :-1])[1:] == (24, 10, 6, 70, 10)
+    assert _tensors.row_layout(x[:, :, 2:9])[1:] == (28, 7, 7, 70, 10)
+    assert _tensors.row_layout(x[1])[1:] == (7, 10, 7, 0, 10)
+    assert _tensors.row_layout(x[1, 2])[1:] == (1, 10, 1, 0, 10)
+    turned = _tensors.row_layout(x.transpose(1, 2))
     assert turned[0].is_contiguous() and turned[1:] == (40, 7, 40, 0, 7)
-    assert F.row_layout(torch.zeros(2, 3, 4, 5))[1:] == (24, 5, 24, 0, 5)
-    assert F.row_layout(torch.zeros(0, 5))[1:4] == (0, 5, 1)
+    assert _tensors.row_layout(torch.zeros(2, 3, 4, 5))[1:] == (24, 5, 24, 0, 5)
+    assert _tensors.row_layout(torch.zeros(0, 5))[1:4] == (0, 5, 1)
 
 
 def test_dense():
     x = torch.zeros(4, 6, 5)
     for t, dense in ((x, True), (x.permute(2, 0, 1), True), (x[:, :3], False), (x[:, ::2], False), (x[:1].expand(4, 6, 5), False),
                      (x[:1], True), (x[:, :1, :1], False), (x[:0, :3], True), (torch.zeros(()), True)):
-        assert OF.is_dense(t) is dense
+        assert _tensors.is_dense(t) is dense
 
 
 def logprobs(rows=2, n=8, inner=2, x=0x1000, code=0, target=0x2000, bits=64, temperature=1.0, logprob=0x3000, entropy=0, stats=0):
     C.token_logprobs_forward_launcher(rows, n, inner, 0, n, x, code, target, bits, -100, temperature, logprob, entropy, stats, 0)
 
 
-def test_tensors_read_by_the_library():
-    """Lists it does not take (on the CPU, strided, of other types) are left to the slower reading, without an error."""
-    cpu = [torch.zeros(3), torch.zeros(4, requires_grad=True)]
-    assert C.clip_table_from_tensors(cpu, cpu) is None
-    assert C.clip_table_from_tensors([], []) is None
-    assert C.clip_table_from_tensors([1.0], [1.0]) is None
-    assert C.clip_table_from_tensors([None], [None]) is None
-    assert C.clip_table_from_tensors([torch.zeros(2, 3).t()], [torch.zeros(6)]) is None
-    assert C.clip_table_from_tensors([torch.zeros(3, dtype=torch.complex64).conj()], [torch.zeros(3)]) is None
-    assert C.clip_table_from_tensors((torch.zeros(3),), (torch.zeros(3),)) is None
-    assert C.clip_table_from_tensors([torch.zeros(3)], []) is None
-    with pytest.raises((RuntimeError, ValueError, BufferError, AssertionError)):
-        clip_grads([torch.zeros(3).to_sparse()], 1.0)
+def test_tensors_that_are_none():
+    """What is no plain tensor of numbers is refused, not read."""
+    for bad in (torch.zeros(3).to_sparse(), torch.zeros(3, device="meta"), torch.zeros(3, dtype=torch.complex64).conj(), 1.0, "grad"):
+        with pytest.raises((RuntimeError, ValueError, TypeError, AssertionError)):
+            clip_grads([bad], 1.0)
+        with pytest.raises((RuntimeError, ValueError, TypeError, AssertionError)):
+            PolicyLoss()(bad, bad, bad)
+        with pytest.raises((RuntimeError, ValueError, TypeError, AssertionError)):
+            PreferenceLoss()(bad)
+        with pytest.raises((RuntimeError, ValueError, TypeError, AssertionError)):
+            TokenLogProbs()(bad, torch.zeros(3, dtype=torch.long))
+    with pytest.raises(TypeError):
+        PolicyLoss()(torch.zeros(2, 3), None, torch.zeros(2))
 
 
 def test_clip_grads_without_an_output():
