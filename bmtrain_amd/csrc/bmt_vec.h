@@ -105,16 +105,19 @@ __device__ __forceinline__ void store4(typename Elem<T>::Bits *p, int count, con
     }
 }
 // Four consecutive elements as raw bits, to be converted later: loads of several arrays can be on their way before the
-// first value is needed.  load: all four exist; load_some: the first `count` do, the others read as 0.
+// first value is needed.  load: all four exist (PAST: read past the caches); load_some: the first `count` do, the others read as 0.
 template <typename T>
 struct Raw4 {
     uint32_t w[sizeof(typename Elem<T>::Bits)];        // 2 dwords of 16-bit elements, 4 of 32-bit ones
+    template <bool PAST = false>
     __device__ __forceinline__ void load(const typename Elem<T>::Bits *p) {
         if (sizeof(typename Elem<T>::Bits) == 2) {
-            const u32x2 v = *(const u32x2_any2 *)p;
+            const u32x2_any2 *at = (const u32x2_any2 *)p;
+            const u32x2 v = PAST ? __builtin_nontemporal_load(at) : *at;
             w[0] = v[0], w[1] = v[1];
         } else {
-            const u32x4 v = *(const u32x4_any4 *)p;
+            const u32x4_any4 *at = (const u32x4_any4 *)p;
+            const u32x4 v = PAST ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
             for (int k = 0; k < (int)sizeof(typename Elem<T>::Bits); k++) w[k] = v[k];
         }

@@ -17,8 +17,10 @@
 // token's unweighted derivative; one workgroup adds the sums in a fixed order; the backward pass multiplies by weight and
 // upstream.  Four neighbouring tokens are added in fp32, everything above in 64 bits.  All of a quad's loads are asked for
 // before the first value is used; values that few tokens need (|x| >= 1, ties at a border) are computed behind a branch
-// of the whole wave.  Bound by HBM and the latency of its loads for large batches (1,024 x 8,192 fp32 with reference and
-// entropy: 176 MB in 40 us, 4.4 TB/s; 107 registers leave four waves to a SIMD, and fewer spill), by launches for small.
+// of the whole wave.  A masked token counts as d = q = A = 0, which adds nothing anywhere; the borders and the ratios they
+// cut to are picked by the advantage's sign, once for a row with one advantage.  Bound by HBM and the latency of its loads
+// for large batches (1,024 x 8,192 fp32 with reference and entropy: 176 MB in 35.5 us, 5.0 TB/s; 95 to 111 registers leave
+// four waves to a SIMD, a cap for five makes them spill: 50 us for both launches instead of 40.6), by launches for small.
 #include "bmt_vec.h"
 #include "../../include/bmt_hip.h"
 
@@ -57,6 +59,16 @@ __device__ __forceinline__ float exp_tail_series(float x) {
     return x * x * s;
 }
 
+// On which side of 1 a token's ratio is cut, by the sign of its advantage: above `high` to `ratio`, below `low`.
+struct Side {
+    float high, low, ratio;
+};
+__device__ __forceinline__ Side side_of(const PolicyIn &in, float A) {
+    if (A > 0.f) return {(float)in.high, -INFINITY, in.ratio_high};
+    if (A < 0.f) return {(float)in.far, (float)in.low, in.ratio_far};
+    return {INFINITY, -INFINITY, 1.f};
+}
+
 template <typename T>
 struct Tokens {                      // four tokens as they are in memory
     Raw4<T> logprob, old, ref, entropy;
@@ -78,20 +90,21 @@ __device__ __forceinline__ void workgroup_sums(double *v, double (*slots)[8], do
     __syncthreads();
 }
 
-// kWhole: the workgroup's lanes work on one unit; kGroups: groups of in.lanes lanes of a wave do; kTiny: the same for rows of
+// COL: one advantage for each token, not one for a row.  kWhole: the workgroup's lanes work on one unit; kGroups: groups of in.lanes lanes of a wave do; kTiny: the same for rows of
 // up to three tokens.
 enum Form { kWhole, kGroups, kTiny };
-template <typename T, Form FORM>
+template <typename T, Form FORM, bool COL>
 __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, uint32_t units, float *__restrict__ saved,
                                                                    float *__restrict__ weights, double *__restrict__ sums) {
     typedef typename Elem<T>::Bits Bits;
-    constexpr bool WHOLE = FORM == kWhole;
+    // Long fp32 rows are read past the caches, which leaves them to what the backward pass reads: 8.4 M tokens with reference
+    // and entropy 40.6 / 43.4 us past / through the caches, both launches; bf16 without entropy 27.6 / 26.4.
+    constexpr bool WHOLE = FORM == kWhole, PAST = WHOLE && sizeof(Bits) == 4;
     const int lanes = WHOLE ? kLossThreads : in.lanes, groups = kLossThreads / lanes;
     const int lane = threadIdx.x % lanes, group = WHOLE ? 0 : threadIdx.x / lanes, step = lanes * 4;
     const bool split = in.chunks > 1;
     __shared__ double slots[kLossThreads / kWave][8], all[8];
     double total[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const float high = (float)in.high, low = (float)in.low, far = (float)in.far;
     for (uint32_t first = blockIdx.x * groups; first < units; first += gridDim.x * groups) {
         const uint32_t unit = first + group;
         const bool there = unit < units;
@@ -104,7 +117,9 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
         const Bits *ep = (const Bits *)in.entropy + row * in.entropy_row;
         const uint8_t *mp = in.mask ? in.mask + row * in.mask_row : nullptr;
         const float *ap = in.advantage + row * in.advantage_row;
-        const float row_advantage = there && !in.advantage_col ? ap[0] : 0.f;
+        const float row_advantage = there && !COL ? ap[0] : 0.f;
+        const Side row_side = side_of(in, row_advantage);
+        int clipped = 0, tokens = 0;
         double acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         for (int i = begin + lane * 4; i < end; i += step) {
             // The last quad of a row that has fewer than four tokens left starts further in front and leaves out what it
@@ -117,56 +132,60 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
                 now.old.load_some(op + at, end - at);
                 now.ref.load_some(fp + at, end - at);
                 if (in.entropy) now.entropy.load_some(ep + at, end - at);
-                if (in.advantage_col) now.advantage.load_some((const uint32_t *)ap + at, end - at);
+                if (COL) now.advantage.load_some((const uint32_t *)ap + at, end - at);
             } else {
                 now.mask = mp ? *(const u32_any1 *)(mp + at) : 0x01010101u;
-                now.logprob.load(lp + at);
-                now.old.load(op + at);
-                now.ref.load(fp + at);
-                if (in.entropy) now.entropy.load(ep + at);
-                if (in.advantage_col) now.advantage.load((const uint32_t *)ap + at);
+                now.logprob.template load<PAST>(lp + at);
+                now.old.template load<PAST>(op + at);
+                now.ref.template load<PAST>(fp + at);
+                if (in.entropy) now.entropy.template load<PAST>(ep + at);
+                if (COL) now.advantage.load((const uint32_t *)ap + at);
                 now.mask &= 0xFFFFFFFFu << (8 * skip);
             }
-            float sum[5] = {0, 0, 0, 0, 0};               // of these four tokens
-            float g[4], most = 0.f;
-            bool tie = false;
+            float sum[4] = {0, 0, 0, 0};                  // of these four tokens: policy, kl, entropy, old_kl
+            float g[4], d[4], q[4], A[4], most = 0.f;
+            bool on[4], tie = false;
+            Side side[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float l = now.logprob.get(k), d = l - now.old.get(k);
-                const float A = in.advantage_col ? now.advantage.get(k) : row_advantage;
-                most = fmaxf(most, fmaxf(fabsf(d), fabsf(now.ref.get(k) - l)));
-                tie |= d == high || d == low || d == far || !(d == d) || !(A == A);
-            }
-            const bool plain = !__any(!(most < 1.f) || tie);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float l = now.logprob.get(k), o = now.old.get(k), d = l - o, q = now.ref.get(k) - l;
-                const float A = in.advantage_col ? now.advantage.get(k) : row_advantage;
-                float old_kl = exp_tail_series(d), rm1 = d + old_kl;       // e^d - 1 - d, e^d - 1
-                float kl = exp_tail_series(q), qm1 = q + kl;
+                // what is masked counts as d = q = A = 0, which adds nothing anywhere
+                const float l = now.logprob.get(k);
+                on[k] = mask_set(now.mask, k);
+                d[k] = on[k] ? l - now.old.get(k) : 0.f;
+                q[k] = on[k] ? now.ref.get(k) - l : 0.f;
+                A[k] = on[k] ? COL ? now.advantage.get(k) : row_advantage : 0.f;
+                side[k] = COL ? side_of(in, A[k]) : row_side;
+                most = fmaxf(most, fmaxf(fabsf(d[k]), fabsf(q[k])));
                 // rounding keeps the order, so the rounded d against a rounded border is the answer unless they are equal
-                bool over = A > 0.f ? d > high : A < 0.f && d > far, under = A < 0.f && d < low;
-                if (!plain) {
-                    const double wide = (double)l - (double)o;
-                    over = A > 0.f ? wide > in.high : A < 0.f && wide > in.far;
-                    under = A < 0.f && wide < in.low;
-                    if (!(fabsf(d) < 1.f)) rm1 = expf(d) - 1.f, old_kl = rm1 - d;
-                    if (!(fabsf(q) < 1.f)) qm1 = expf(q) - 1.f, kl = qm1 - q;
-                }
-                const float r = over ? (A > 0.f ? in.ratio_high : in.ratio_far) : under ? in.ratio_low : 1.f + rm1;
-                const float policy = -r * A;
-                const float slope = (over || under ? 0.f : policy) - (in.kl_coef != 0.f ? in.kl_coef * qm1 : 0.f);
-                const bool on = mask_set(now.mask, k);
-                g[k] = on ? slope : 0.f;
-                sum[0] += on ? policy : 0.f;
-                sum[1] += on ? kl : 0.f;
-                sum[2] += on && in.entropy ? now.entropy.get(k) : 0.f;
-                sum[3] += on && (over || under) ? 1.f : 0.f;
-                sum[4] += on ? old_kl : 0.f;
+                tie |= d[k] == side[k].high || d[k] == side[k].low;
             }
+            const bool careful = __any(!(most < 1.f) || tie);
 #pragma unroll
-            for (int k = 0; k < 5; k++) acc[k] += (double)sum[k];
-            acc[5] += (double)mask_count(now.mask);
+            for (int k = 0; k < 4; k++) {
+                float old_kl = exp_tail_series(d[k]), rm1 = d[k] + old_kl;       // e^d - 1 - d, e^d - 1
+                float kl = exp_tail_series(q[k]), qm1 = q[k] + kl;
+                bool over = d[k] > side[k].high, under = d[k] < side[k].low;
+                if (careful) {
+                    const double wide = on[k] ? (double)now.logprob.get(k) - (double)now.old.get(k) : 0.0;
+                    over = A[k] > 0.f ? wide > in.high : A[k] < 0.f && wide > in.far;
+                    under = A[k] < 0.f && wide < in.low;
+                    if (!(fabsf(d[k]) < 1.f)) rm1 = expf(d[k]) - 1.f, old_kl = rm1 - d[k];
+                    if (!(fabsf(q[k]) < 1.f)) qm1 = expf(q[k]) - 1.f, kl = qm1 - q[k];
+                }
+                const float r = over ? side[k].ratio : under ? in.ratio_low : 1.f + rm1;
+                const float policy = -r * A[k];
+                g[k] = (over || under ? 0.f : policy) - (in.kl_coef != 0.f ? in.kl_coef * qm1 : 0.f);
+                sum[0] += policy;
+                sum[1] += kl;
+                if (in.entropy) sum[2] += on[k] ? now.entropy.get(k) : 0.f;
+                sum[3] += old_kl;
+                clipped += over || under ? 1 : 0;
+                tokens += on[k] ? 1 : 0;
+            }
+            acc[0] += (double)sum[0];
+            acc[1] += (double)sum[1];
+            if (in.entropy) acc[2] += (double)sum[2];
+            acc[4] += (double)sum[3];
             if (saved) {
                 uint32_t *to = (uint32_t *)saved + row * in.time + at;
                 if (FORM == kTiny) {
@@ -180,6 +199,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
                 }
             }
         }
+        acc[3] = clipped, acc[5] = tokens;
         if (!split && in.reduction == kSequence) {        // the row is this group's: its own mean
             if (WHOLE) {
                 workgroup_sums(acc, slots, all);
@@ -278,8 +298,8 @@ struct Shape {
 // A row of up to 256 tokens is that of 8 to 64 lanes, four tokens each; up to 1,024 it is a workgroup's while there are few
 // rows, where it is the latency that counts, and a wave's when there are many.  Longer rows are split into parts of a
 // workgroup each, the shortest from 1,024 to 16,384 tokens that give at most 1,024 parts: a workgroup's start and its
-// sums cost as much as some 2,000 tokens (8.4 M tokens fp32 with reference and entropy: 45 us in parts of 8,192 tokens,
-// 48 of 4,096, 51 of 2,048, 66 of 1,024; both launches).
+// sums cost as much as some 2,000 tokens (8.4 M tokens fp32 with reference and entropy: 40.6 us in parts of 8,192 tokens,
+// 42.3 of 4,096, 46.4 of 2,048, 63 of 1,024; both launches).
 static Shape shape_of(int64_t rows, int64_t time) {
     Shape s;
     s.unit = 1024;
@@ -295,17 +315,20 @@ static Shape shape_of(int64_t rows, int64_t time) {
     return s;
 }
 
-template <typename T>
+template <typename T, bool COL>
 static void loss_launch(const PolicyIn &in, const Shape &s, float *saved, float *weights, double *sums, hipStream_t stream) {
+    const dim3 grid((unsigned)s.grid), threads(kLossThreads);
     if (s.lanes == kLossThreads)
-        hipLaunchKernelGGL((policy_loss_kernel<T, kWhole>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
-                           saved, weights, sums);
+        hipLaunchKernelGGL((policy_loss_kernel<T, kWhole, COL>), grid, threads, 0, stream, in, (uint32_t)s.units, saved, weights, sums);
     else if (in.time >= 4)
-        hipLaunchKernelGGL((policy_loss_kernel<T, kGroups>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
-                           saved, weights, sums);
+        hipLaunchKernelGGL((policy_loss_kernel<T, kGroups, COL>), grid, threads, 0, stream, in, (uint32_t)s.units, saved, weights, sums);
     else
-        hipLaunchKernelGGL((policy_loss_kernel<T, kTiny>), dim3((unsigned)s.grid), dim3(kLossThreads), 0, stream, in, (uint32_t)s.units,
-                           saved, weights, sums);
+        hipLaunchKernelGGL((policy_loss_kernel<T, kTiny, COL>), grid, threads, 0, stream, in, (uint32_t)s.units, saved, weights, sums);
+}
+template <typename T>
+static void loss_pick(const PolicyIn &in, const Shape &s, float *saved, float *weights, double *sums, hipStream_t stream) {
+    if (in.advantage_col) loss_launch<T, true>(in, s, saved, weights, sums, stream);
+    else loss_launch<T, false>(in, s, saved, weights, sums, stream);
 }
 
 static bool fits(int64_t rows, int64_t time) {
@@ -360,9 +383,9 @@ extern "C" int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t 
         in.far = dual_clip != 0 ? log(dual_clip) : (double)INFINITY;
         in.ratio_high = (float)(1 + clip_high), in.ratio_low = (float)(1 - clip_low), in.ratio_far = (float)dual_clip;
         in.kl_coef = kl_coef;
-        if (type == kFp32) loss_launch<Single>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
-        else if (type == kFp16) loss_launch<Half>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
-        else loss_launch<BFloat16>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
+        if (type == kFp32) loss_pick<Single>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
+        else if (type == kFp16) loss_pick<Half>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
+        else loss_pick<BFloat16>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return fail((int)e, who, e);
     }
