@@ -10,9 +10,9 @@
 //
 // Squares are formed and added in 64 bits: an fp32 or bf16 gradient's square may lie outside fp32's range.  Partial
 // sums, one to a tile, are added in a fixed order: equal inputs give equal bits.
-// Up to kBatch tensors of one pair of types travel in a launch's arguments; tiles are numbered through the tensors and
-// a workgroup finds its tensor there.  The second pass goes through the gradients backwards, from what the first one
-// read last, and both read and write past the caches (non-temporal).
+// Up to kBatch tensors travel in a launch's arguments, whatever their types; tiles are numbered through the tensors and
+// a workgroup finds its tensor and its types there.  The second pass goes through the gradients backwards, from what the
+// first one read last, and both read and write past the caches (non-temporal).
 // Measured on 45 fp32 tensors of 1.01 B elements into bf16: norm 0.59 ms (6.9 TB/s; 0.66 ms with temporal loads, 0.66
 // with half the tile), scaling 0.91 ms (6.7 TB/s; 0.95 with one tile to an XCD in turn, 0.98 with three vectors to a
 // lane); 202 M bf16 elements 64 + 128 us.  Leaving the first pass's last 128 to 240 MiB to the cache changed nothing, runs
@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 namespace bmt {
@@ -39,6 +40,7 @@ struct Batch {
     void *dst[kBatch];
     int64_t n[kBatch];
     uint32_t first[kBatch];              // number of a tensor's first tile; 0xFFFFFFFF behind the last tensor
+    uint8_t types[kBatch];               // src_type + 4 * dst_type
 };
 
 // The tensor of tile `tile`: the last one that starts at or in front of it (a bisection over the arguments).
@@ -62,14 +64,30 @@ __device__ __forceinline__ void norm_add(double &acc, float &top, uint32_t &nan,
     }
 }
 
+// The sum, or the larger one; a NaN stays.
+template <bool MAX>
+__device__ __forceinline__ double join(double a, double b) {
+    return MAX ? a != a ? a : b > a || b != b ? b : a : a + b;
+}
+// Over a workgroup of kThreads, in a fixed order; thread 0 has it.
+template <bool MAX>
+__device__ __forceinline__ double workgroup_join(double acc) {
+    __shared__ double slots[kThreads / kWave];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) acc = join<MAX>(acc, __shfl_xor(acc, off, kWave));
+    if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int k = 1; k < kThreads / kWave; k++) acc = join<MAX>(acc, slots[k]);
+    return acc;
+}
+
+// The tensor's tile into the thread's sum, or largest magnitude (NaN where there is one).
 template <typename T, bool MAX>
-__global__ __launch_bounds__(kThreads) void grad_norm_kernel(Batch batch, double *__restrict__ partials) {
+__device__ __forceinline__ double norm_tile(const void *src, int64_t n, uint32_t tile) {
     typedef Elem<T> E;
     constexpr int K = E::kVec;
-    const int which = find_tensor(batch, blockIdx.x);
-    const typename E::Bits *g = (const typename E::Bits *)batch.src[which];
-    const int64_t n = batch.n[which];
-    const uint32_t tile = blockIdx.x - batch.first[which];
+    const typename E::Bits *g = (const typename E::Bits *)src;
     const int head = head_elements<T>(g, n < 64 ? (int)n : 64);
     const int64_t nvec = (n - head) / K;
     const u32x4 *body = (const u32x4 *)(g + head);
@@ -95,22 +113,19 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(Batch batch, double
         if ((int64_t)threadIdx.x < edge)
             norm_add<MAX>(acc, top, nan, E::get(g[(int64_t)threadIdx.x < head ? (int64_t)threadIdx.x : tail_lo + threadIdx.x - head]));
     }
-    if (MAX) acc = nan ? (double)__builtin_nanf("") : (double)top;
-    __shared__ double slots[kThreads / kWave];
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const double other = __shfl_xor(acc, off, kWave);
-        acc = MAX ? (acc != acc ? acc : other > acc || other != other ? other : acc) : acc + other;
-    }
-    if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = acc;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < kThreads / kWave; k++) {
-            const double other = slots[k];
-            acc = MAX ? (acc != acc ? acc : other > acc || other != other ? other : acc) : acc + other;
-        }
-        partials[blockIdx.x] = acc;
-    }
+    return MAX ? nan ? (double)__builtin_nanf("") : (double)top : acc;
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(Batch batch, double *__restrict__ partials) {
+    const int which = find_tensor(batch, blockIdx.x);
+    const uint32_t tile = blockIdx.x - batch.first[which];
+    const int type = batch.types[which] & 3;
+    double acc = type == kFp32   ? norm_tile<Single, MAX>(batch.src[which], batch.n[which], tile)
+                 : type == kFp16 ? norm_tile<Half, MAX>(batch.src[which], batch.n[which], tile)
+                                 : norm_tile<BFloat16, MAX>(batch.src[which], batch.n[which], tile);
+    acc = workgroup_join<MAX>(acc);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
 // out: n / scale, then the factor c.
@@ -118,21 +133,8 @@ template <bool MAX>
 __global__ __launch_bounds__(kThreads) void grad_norm_finish_kernel(const double *__restrict__ partials, int64_t count, double max_norm,
                                                                     double eps, double scale, float *__restrict__ out) {
     double acc = 0;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) {
-        const double other = partials[i];
-        acc = MAX ? (acc != acc ? acc : other > acc || other != other ? other : acc) : acc + other;
-    }
-    __shared__ double lanes[kThreads];
-    lanes[threadIdx.x] = acc;
-    __syncthreads();
-    for (int stride = kThreads / 2; stride > 0; stride >>= 1) {
-        if ((int)threadIdx.x < stride) {
-            const double other = lanes[threadIdx.x + stride];
-            acc = MAX ? (acc != acc ? acc : other > acc || other != other ? other : acc) : acc + other;
-            lanes[threadIdx.x] = acc;
-        }
-        __syncthreads();
-    }
+    for (int64_t i = threadIdx.x; i < count; i += kThreads) acc = join<MAX>(acc, partials[i]);
+    acc = workgroup_join<MAX>(acc);
     if (threadIdx.x == 0) {
         const double norm = MAX ? acc : sqrt(acc);
         out[0] = (float)(norm / scale);
@@ -154,23 +156,16 @@ __device__ __forceinline__ void store_past_cache(typename Elem<D>::Bits *to, con
     }
 }
 
-// The factor a tensor is multiplied by: c, or c rounded to the tensor's type (what torch's multiplication of a 16-bit
-// tensor by a 0-dim fp32 tensor does); 1 where c is not below 1, a NaN among them.
+// The tensor's tile times f.
 template <typename S, typename D>
-__global__ __launch_bounds__(kScaleThreads) void grad_scale_kernel(Batch batch, const float *__restrict__ coef, int32_t round_coef) {
+__device__ __forceinline__ void scale_tile(const void *src, void *dst, int64_t n, int64_t number, float c, int32_t round_coef) {
     typedef Elem<S> E;
     constexpr int K = E::kVec;
-    const float c = coef[0];
-    const bool scales = c < 1.f;
-    const uint32_t number = xcd_run<kScaleRun>(blockIdx.x, gridDim.x);
-    const int which = find_tensor(batch, number);
-    const typename E::Bits *g = (const typename E::Bits *)batch.src[which];
-    typename Elem<D>::Bits *o = (typename Elem<D>::Bits *)batch.dst[which];
-    if (!scales && (const void *)g == (const void *)o) return;
-    const float f = !scales ? 1.f : round_coef ? E::get(E::put(c)) : c;
-    const int64_t n = batch.n[which];
+    const typename E::Bits *g = (const typename E::Bits *)src;
+    typename Elem<D>::Bits *o = (typename Elem<D>::Bits *)dst;
+    const float f = !(c < 1.f) ? 1.f : round_coef ? E::get(E::put(c)) : c;
     constexpr int64_t kTile = (int64_t)kScaleThreads * kScaleUnroll;       // vectors
-    const int64_t tile = (n + kTile * K - 1) / (kTile * K) - 1 - (number - batch.first[which]);      // last tile first
+    const int64_t tile = (n + kTile * K - 1) / (kTile * K) - 1 - number;   // last tile first
     const int head = head_elements<S>(g, n < 64 ? (int)n : 64);
     const int64_t nvec = (n - head) / K;
     const u32x4 *body = (const u32x4 *)(g + head);
@@ -198,6 +193,45 @@ __global__ __launch_bounds__(kScaleThreads) void grad_scale_kernel(Batch batch, 
     }
 }
 
+template <typename S>
+__device__ __forceinline__ void scale_tile_into(int dst_type, const void *src, void *dst, int64_t n, int64_t number, float c, int32_t round_coef) {
+    if (dst_type == kFp32) scale_tile<S, Single>(src, dst, n, number, c, round_coef);
+    else if (dst_type == kFp16) scale_tile<S, Half>(src, dst, n, number, c, round_coef);
+    else scale_tile<S, BFloat16>(src, dst, n, number, c, round_coef);
+}
+
+// The factor a tensor is multiplied by: c, or c rounded to the tensor's type (what torch's multiplication of a 16-bit
+// tensor by a 0-dim fp32 tensor does); 1 where c is not below 1, a NaN among them.  TYPES: those of all tensors of the
+// launch, or kMixed (one launch instead of up to nine: a call on 36 small tensors of three types into three types 16 us
+// instead of 56; where all are alike the types are the compiler's, 1.01 B fp32 elements into bf16 0.91 ms instead of 0.94).
+constexpr int kMixed = -1;
+template <int TYPES>
+__global__ __launch_bounds__(kScaleThreads) void grad_scale_kernel(Batch batch, const float *__restrict__ coef, int32_t round_coef) {
+    const float c = coef[0];
+    const uint32_t unit = xcd_run<kScaleRun>(blockIdx.x, gridDim.x);
+    const int which = find_tensor(batch, unit);
+    const void *src = batch.src[which];
+    void *dst = batch.dst[which];
+    if (!(c < 1.f) && src == (const void *)dst) return;
+    const int types = TYPES == kMixed ? batch.types[which] : TYPES, src_type = types & 3, dst_type = types >> 2;
+    const int64_t n = batch.n[which], number = unit - batch.first[which];
+    if (src_type == kFp32) scale_tile_into<Single>(dst_type, src, dst, n, number, c, round_coef);
+    else if (src_type == kFp16) scale_tile_into<Half>(dst_type, src, dst, n, number, c, round_coef);
+    else scale_tile_into<BFloat16>(dst_type, src, dst, n, number, c, round_coef);
+}
+
+template <int... TYPES>
+void scale_launch(std::integer_sequence<int, TYPES...>, const Batch &b, uint32_t tiles, int types, const float *coef, int32_t round_coef,
+                  hipStream_t s) {
+    auto one = [&](auto t) {
+        constexpr int kTypes = decltype(t)::value;
+        if (types != kTypes) return false;
+        hipLaunchKernelGGL((grad_scale_kernel<kTypes>), dim3(tiles), dim3(kScaleThreads), 0, s, b, coef, round_coef);
+        return true;
+    };
+    (one(std::integral_constant<int, TYPES>()) || ...);
+}
+
 uintptr_t size_of(int32_t type) { return type == kFp32 ? 4 : 2; }
 bool known(int32_t type) { return type == kFp32 || type == kFp16 || type == kBf16; }
 // Tiles of `vectors` 16-byte vectors.
@@ -207,29 +241,30 @@ int64_t tiles_of(const bmt_clip_tensor &t, int64_t vectors) {
 }
 constexpr int64_t kNormTile = (int64_t)kThreads * kUnroll, kScaleTile = (int64_t)kScaleThreads * kScaleUnroll;
 
-// Calls launch(batch, tiles) for batches of the tensors with these types (dst_type < 0: any), in order or backwards.
+// Calls launch(batch, tiles, the types of all its tensors or kMixed) for batches of the tensors, in order or backwards.
 template <typename F>
-hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, int64_t vectors, int threads,
-                      bool backwards, F launch) {
+hipError_t in_batches(int32_t count, const bmt_clip_tensor *tensors, int64_t vectors, int threads, bool backwards, F launch) {
     Batch b;
-    int held = 0;
+    int held = 0, types = kMixed;
     int64_t tiles = 0;
     auto flush = [&]() -> hipError_t {
         if (!held) return hipSuccess;
-        for (int k = held; k < kBatch; k++) b.src[k] = nullptr, b.dst[k] = nullptr, b.n[k] = 0, b.first[k] = 0xFFFFFFFFu;
-        launch(b, (uint32_t)tiles);
+        for (int k = held; k < kBatch; k++) b.src[k] = nullptr, b.dst[k] = nullptr, b.n[k] = 0, b.first[k] = 0xFFFFFFFFu, b.types[k] = 0;
+        launch(b, (uint32_t)tiles, types);
         held = 0, tiles = 0;
         return hipGetLastError();
     };
     for (int32_t j = 0; j < count; j++) {
         const bmt_clip_tensor &t = tensors[backwards ? count - 1 - j : j];
-        if (t.n <= 0 || t.src_type != src_type || (dst_type >= 0 && t.dst_type != dst_type)) continue;
+        if (t.n <= 0) continue;
         const int64_t more = tiles_of(t, vectors);
         if (held == kBatch || !launch_fits(tiles + more, threads)) {
             const hipError_t e = flush();
             if (e != hipSuccess) return e;
         }
         b.src[held] = t.src, b.dst[held] = t.dst, b.n[held] = t.n, b.first[held] = (uint32_t)tiles;
+        b.types[held] = (uint8_t)(t.src_type + 4 * (t.dst_type & 3));
+        types = held == 0 || types == b.types[held] ? b.types[held] : kMixed;
         tiles += more;
         held++;
     }
@@ -282,31 +317,6 @@ const char *check_overlap(int32_t count, const bmt_clip_tensor *tensors) {
     return nullptr;
 }
 
-template <typename S>
-hipError_t norm_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t type, bool max, double *partials, int64_t *used,
-                       hipStream_t s) {
-    return in_batches(count, tensors, type, -1, kNormTile, kThreads, false, [&](const Batch &b, uint32_t tiles) {
-        if (max) hipLaunchKernelGGL((grad_norm_kernel<S, true>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
-        else hipLaunchKernelGGL((grad_norm_kernel<S, false>), dim3(tiles), dim3(kThreads), 0, s, b, partials + *used);
-        *used += tiles;
-    });
-}
-
-template <typename S, typename D>
-hipError_t scale_passes(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, int32_t dst_type, const float *coef,
-                        int32_t round_coef, hipStream_t s) {
-    return in_batches(count, tensors, src_type, dst_type, kScaleTile, kScaleThreads, true, [&](const Batch &b, uint32_t tiles) {
-        hipLaunchKernelGGL((grad_scale_kernel<S, D>), dim3(tiles), dim3(kScaleThreads), 0, s, b, coef, round_coef);
-    });
-}
-template <typename S>
-hipError_t scale_from(int32_t count, const bmt_clip_tensor *tensors, int32_t src_type, const float *coef, int32_t round_coef, hipStream_t s) {
-    hipError_t e = scale_passes<S, Single>(count, tensors, src_type, kFp32, coef, round_coef, s);
-    if (e == hipSuccess) e = scale_passes<S, Half>(count, tensors, src_type, kFp16, coef, round_coef, s);
-    if (e == hipSuccess) e = scale_passes<S, BFloat16>(count, tensors, src_type, kBf16, coef, round_coef, s);
-    return e;
-}
-
 }  // namespace
 }  // namespace bmt
 
@@ -328,9 +338,11 @@ extern "C" int grad_norm_multi_launcher(int32_t count, const bmt_clip_tensor *te
     hipStream_t s = (hipStream_t)stream;
     double *partials = (double *)workspace;
     int64_t used = 0;
-    hipError_t e = norm_passes<Single>(count, tensors, kFp32, use_max != 0, partials, &used, s);
-    if (e == hipSuccess) e = norm_passes<Half>(count, tensors, kFp16, use_max != 0, partials, &used, s);
-    if (e == hipSuccess) e = norm_passes<BFloat16>(count, tensors, kBf16, use_max != 0, partials, &used, s);
+    hipError_t e = in_batches(count, tensors, kNormTile, kThreads, false, [&](const Batch &b, uint32_t tiles, int) {
+        if (use_max) hipLaunchKernelGGL((grad_norm_kernel<true>), dim3(tiles), dim3(kThreads), 0, s, b, partials + used);
+        else hipLaunchKernelGGL((grad_norm_kernel<false>), dim3(tiles), dim3(kThreads), 0, s, b, partials + used);
+        used += tiles;
+    });
     if (e != hipSuccess) return fail((int)e, who, e);
     if (use_max)
         hipLaunchKernelGGL((grad_norm_finish_kernel<true>), dim3(1), dim3(kThreads), 0, s, partials, used, max_norm, eps, scale, (float *)out);
@@ -354,8 +366,8 @@ extern "C" int grad_scale_multi_launcher(int32_t count, const bmt_clip_tensor *t
         return refuse(who, "out of host memory");
     }
     hipStream_t s = (hipStream_t)stream;
-    hipError_t e = scale_from<BFloat16>(count, tensors, kBf16, (const float *)coef, round_coef, s);     // backwards here too
-    if (e == hipSuccess) e = scale_from<Half>(count, tensors, kFp16, (const float *)coef, round_coef, s);
-    if (e == hipSuccess) e = scale_from<Single>(count, tensors, kFp32, (const float *)coef, round_coef, s);
+    const hipError_t e = in_batches(count, tensors, kScaleTile, kScaleThreads, true, [&](const Batch &b, uint32_t tiles, int types) {
+        scale_launch(std::integer_sequence<int, kMixed, 0, 1, 2, 4, 5, 6, 8, 9, 10>(), b, tiles, types, (const float *)coef, round_coef, s);
+    });
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }
