@@ -71,8 +71,14 @@ void launched(const char *who, int status) {
 Tensor floats(at::IntArrayRef shape, const Tensor &like) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Forward-mode derivatives would be lost without a word.
+void no_tangent(const Tensor &t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "forward-mode differentiation is not supported");
+}
+
 // `t` with its last dimension's elements next to each other (a copy where they are not).
 Tensor tokens_adjacent(const Tensor &t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();
     return t.dim() == 0 || t.is_contiguous() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 Tensor tokens_adjacent(const MaybeTensor &t) { return t ? tokens_adjacent(*t) : Tensor(); }
@@ -114,8 +120,8 @@ struct Rows {
 };
 Rows rows_of(const Tensor &logits) {
     const int64_t dims = logits.dim(), n = logits.size(-1);
-    if (dims > 3 || (n > 1 && logits.stride(-1) != 1)) {
-        const Tensor copy = logits.contiguous();
+    if (dims > 3 || (n > 1 && logits.stride(-1) != 1) || logits.is_neg()) {
+        const Tensor copy = logits.resolve_neg().contiguous();
         const int64_t rows = n ? copy.numel() / n : 0;
         return {copy, rows, n, std::max<int64_t>(rows, 1), 0, n};
     }
@@ -165,6 +171,7 @@ std::tuple<Tensor, MaybeTensor> token_logprobs(const Tensor &logits, const Tenso
     expect(logits.dim() >= 1 && logits.sizes().slice(0, logits.dim() - 1) == target_in.sizes(),
            "target must have the shape of logits without its last dimension");
     expect(logits.is_cuda(), "logits must be on cuda");
+    no_tangent(logits);
     const int32_t code = type_code("token_logprobs", logits.scalar_type());
     expect(target_in.device() == logits.device(), "target must be on the same cuda device as the logits");
     expect(target_in.scalar_type() == at::kInt || target_in.scalar_type() == at::kLong, "target must be an int or long tensor");
@@ -261,6 +268,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor &logprob_in, const Tensor &o
     }
     expect(logprob_in.is_cuda(), "tensors must be on cuda");
     const Tensor logprob = tokens_adjacent(logprob_in), entropy = tokens_adjacent(entropy_in);      // with their gradients
+    no_tangent(logprob), no_tangent(entropy);
     const bool keep = wants_grad(logprob), entropy_grad = wants_grad(entropy);
     const at::ScalarType type = logprob.scalar_type();
     const int32_t code = type_code("policy_loss", type);
@@ -273,7 +281,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor &logprob_in, const Tensor &o
         const Tensor old = tokens_adjacent(old_in), ref = tokens_adjacent(ref_in);
         mask = as_mask(mask_in);
         if (advantages.scalar_type() != at::kFloat) advantages = advantages.to(at::kFloat);
-        advantages = advantages.dim() == 2 ? tokens_adjacent(advantages) : advantages;
+        advantages = advantages.dim() == 2 ? tokens_adjacent(advantages) : advantages.resolve_neg();
         const bool per_token = advantages.dim() == 2;
         expect(per_token ? advantages.sizes() == logprob.sizes() : advantages.dim() == 1 && advantages.size(0) == rows,
                "advantages must be one to a sequence or one to a token");
@@ -345,6 +353,7 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor &logprob_in, con
     const Tensor logprob = tokens_adjacent(sums ? logprob_in.unsqueeze(1) : logprob_in);             // with its gradient
     expect(logprob.dim() == 2 && logprob.size(0) % 2 == 0, "logprob must be [2 * pairs, tokens]");
     expect(logprob.is_cuda(), "tensors must be on cuda");
+    no_tangent(logprob);
     const at::ScalarType type = logprob.scalar_type();
     const int32_t code = type_code("preference_loss", type);
     const int64_t pairs = logprob.size(0) / 2, time = logprob.size(1);
@@ -396,6 +405,7 @@ std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const 
         row.src_type = type(g), row.dst_type = type(o);
         expect(g.is_cuda() && g.device() == grads[0].device() && o.device() == g.device(), "gradients must be on one cuda device");
         expect(o.numel() == g.numel(), "outputs must have their gradients' numbers of elements");
+        expect(!g.is_neg() && !o.is_neg(), "gradients must not be lazily negated");
         expect(is_dense(g), "gradients must not have gaps nor elements that share memory");
         expect((g.is_contiguous() && o.is_contiguous()) || (g.sizes() == o.sizes() && g.strides() == o.strides()),
                "outputs must have their gradients' strides");

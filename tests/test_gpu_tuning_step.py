@@ -203,6 +203,25 @@ def test_transforms_are_refused():
     for name, call, leaf, _ in calls():
         with pytest.raises(RuntimeError):
             torch.func.grad(call)(leaf)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(torch.stack([leaf, leaf]))
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(torch.autograd.forward_ad.make_dual(leaf, leaf))
+
+
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate is a view whose numbers are the memory's, negated."""
+    for name, call, leaf, _ in calls():
+        z = torch.complex(torch.zeros_like(leaf), -leaf)
+        assert z.conj().imag.is_neg() and torch.equal(z.conj().imag, leaf)
+        x = leaf.clone().requires_grad_()
+        want = call(x)
+        grad, = torch.autograd.grad(want, x)
+        view = z.conj().imag.requires_grad_()
+        got = call(view)
+        assert torch.equal(got, want) and torch.equal(torch.autograd.grad(got, view)[0], grad), name
+    with pytest.raises(AssertionError, match="negated"):
+        bmt.optim.clip_grads([z.conj().imag], 1.0)
 
 
 def test_two_threads_and_streams():
