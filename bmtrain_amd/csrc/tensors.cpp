@@ -82,6 +82,12 @@ Tensor tokens_adjacent(const Tensor &t) {
     return t.dim() == 0 || t.is_contiguous() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 Tensor tokens_adjacent(const MaybeTensor &t) { return t ? tokens_adjacent(*t) : Tensor(); }
+// An upstream gradient as the kernels read it: its numbers in memory, in order.  Complex arithmetic behind an operator hands
+// back lazily negated ones, which contiguous() leaves negated.  The result has to live until its launch.
+Tensor upstream_of(const Tensor &grad) {
+    if (!grad.defined()) return Tensor();
+    return grad.is_neg() ? grad.resolve_neg().contiguous() : grad.contiguous();
+}
 // A bool / uint8 mask as it is; anything else as mask != 0.
 Tensor as_mask(const MaybeTensor &mask) {
     if (!mask) return Tensor();
@@ -145,8 +151,7 @@ struct TokenLogProbsBackward : Node {
             const at::NoGradGuard no_graph;
             const c10::DeviceGuard device(logits.device());
             const Rows r = rows_of(logits);
-            const Tensor grad_logprob = grads[0].defined() ? grads[0].contiguous() : Tensor();
-            const Tensor grad_entropy = of_entropy ? grads[1].contiguous() : Tensor();
+            const Tensor grad_logprob = upstream_of(grads[0]), grad_entropy = of_entropy ? upstream_of(grads[1]) : Tensor();
             out[0] = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
             launched("token_logprobs_backward_launcher",
                      token_logprobs_backward_launcher(r.rows, r.n, r.inner, r.outer_stride, r.inner_stride, r.logits.data_ptr(),
@@ -235,12 +240,13 @@ struct PolicyLossBackward : Node {
         {
             const at::NoGradGuard no_graph;
             const c10::DeviceGuard device(scratch.device());
+            const Tensor upstream = upstream_of(grads[0]);
             for (size_t k = 0; k < out.size(); k++)
                 if (task_should_compute_output(k)) out[k] = at::empty({rows, time}, scratch.options().dtype(type));
             const float *base = (const float *)scratch.data_ptr();
             launched("policy_loss_backward_launcher",
                      policy_loss_backward_launcher(rows, time, code_of(type), reduction, saved_at >= 0 ? base + saved_at : nullptr,
-                                                   base + weights_at, grads[0].data_ptr(), pointer(mask), masked ? mask.stride(0) : 0,
+                                                   base + weights_at, upstream.data_ptr(), pointer(mask), masked ? mask.stride(0) : 0,
                                                    entropy_coef, pointer(out[0]), out.size() > 1 ? pointer(out[1]) : nullptr,
                                                    stream_of(scratch)));
         }
@@ -329,10 +335,11 @@ struct PreferenceLossBackward : Node {
         {
             const at::NoGradGuard no_graph;
             const c10::DeviceGuard device(scratch.device());
+            const Tensor upstream = upstream_of(grads[0]);
             out[0] = at::empty({2 * pairs, time}, scratch.options().dtype(type));
             launched("preference_loss_backward_launcher",
                      preference_loss_backward_launcher(pairs, time, code_of(type), (const float *)scratch.data_ptr() + slope_at,
-                                                       grads[0].data_ptr(), pointer(mask), masked ? mask.stride(0) : 0,
+                                                       upstream.data_ptr(), pointer(mask), masked ? mask.stride(0) : 0,
                                                        out[0].data_ptr(), stream_of(scratch)));
         }
         return once_differentiable(std::move(out), grads);

@@ -243,3 +243,26 @@ def test_two_threads_and_streams():
     [t.join() for t in threads]
     for k in range(2):
         assert all(torch.equal(a, b) for a, b in zip(got[k], want))
+
+
+def test_lazily_negated_upstreams():
+    """An upstream gradient may be a view whose numbers are the memory's, negated: what complex arithmetic behind a loss
+    hands back, and contiguous, so that nothing on the way makes a copy of it."""
+    zero = torch.zeros((), device="cuda")
+    for name, call, leaf, _ in calls():
+        x = leaf.clone().requires_grad_()
+        want, = torch.autograd.grad(call(x), x)
+        (torch.complex(zero, call(x)).conj() * (1 + 2j)).imag.backward()             # the loss's share of it is -1
+        assert torch.equal(x.grad, -want), name
+        got, = torch.autograd.grad(call(x), x, torch._neg_view(torch.ones((), device="cuda")))
+        assert torch.equal(got, -want), name
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for shape in ((4, 7), (1, 1)):
+        x = torch.randn(*shape, 700, generator=gen, device="cuda").requires_grad_()
+        target = torch.randint(0, 700, shape, generator=gen, device="cuda")
+        g, h = [torch.randn(shape, generator=gen, device="cuda") for _ in range(2)]
+        out = bmt.loss.TokenLogProbs(entropy=True)(x, target)
+        want, = torch.autograd.grad(out, x, (-g, -h), retain_graph=True)
+        assert torch._neg_view(g).is_contiguous()
+        got, = torch.autograd.grad(out, x, (torch._neg_view(g), torch._neg_view(h)))
+        assert torch.equal(got, want)
