@@ -202,8 +202,8 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_kernel(
             const float d = (a.m - xt) * c, f = __builtin_amdgcn_exp2f(d), rest = a.s * f;
             if (ENTROPY) a.w = __builtin_fmaf(fmaxf(d, kFar), a.s, a.w) * f;
             a.m = xt, a.s = 1.f + rest;
-            log_sum = log1pf(rest);
-            lp = (xt - xt) - log_sum;                     // NaN for an infinite logit
+            log_sum = log1pf(rest) + (xt - xt);           // NaN for an infinite logit, and with it the entropy and the gradient
+            lp = 0.f - log_sum;
         } else {
             if (inside) online_join<ENTROPY>(a, xt, 1.f, 0.f, c);
             log_sum = logf(a.s);

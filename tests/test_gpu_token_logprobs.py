@@ -330,3 +330,23 @@ def test_confident_tokens_keep_their_digits(dtype, n):
     at_target = grad.double().gather(1, target.unsqueeze(1)).squeeze(1)
     tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126, torch.float32: 2.0 ** -126}[dtype]
     assert ((at_target - rest / (1 + rest)).abs() <= (tol + torch.finfo(dtype).eps / 2 * 1.01) * rest + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 5, 300, 4999, 33000, 131072])
+def test_an_infinite_logit_at_the_target(dtype, n):
+    """A row's only +inf, at the target itself: NaN throughout the row, as with the infinity anywhere else."""
+    places = sorted({0, n // 3, n // 2, n - 1})
+    logits, target, g, h = make(len(places) + 1, n, dtype, n)
+    for r, place in enumerate(places):
+        target[r] = place
+        logits[r, place] = float("inf")
+    bad = torch.arange(len(places) + 1, device="cuda") < len(places)
+    for entropy in (True, False):
+        leaf = logits.clone().requires_grad_()
+        out = TokenLogProbs(entropy=entropy)(leaf, target)
+        out = out if entropy else (out,)
+        grad, = torch.autograd.grad(out, leaf, (g, h)[:len(out)])
+        for t in out:
+            assert torch.equal(torch.isnan(t), bad)
+        assert torch.equal(torch.isnan(grad).all(1), bad) and torch.equal(torch.isnan(grad).any(1), bad)
