@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
         const int end = there ? (in.time - begin < in.unit ? in.time : begin + in.unit) : 0;
         const Bits *lp = (const Bits *)in.logprob + row * in.logprob_row;
         const Bits *op = (const Bits *)in.old + row * in.old_row;
-        const Bits *fp = in.ref ? (const Bits *)in.ref + row * in.ref_row : lp;      // absent: q = 0, nothing comes of it
+        const Bits *fp = in.ref ? (const Bits *)in.ref + row * in.ref_row : lp;      // absent: q is 0, or NaN where l is not finite, and not used
         const Bits *ep = (const Bits *)in.entropy + row * in.entropy_row;
         const uint8_t *mp = in.mask ? in.mask + row * in.mask_row : nullptr;
         const float *ap = in.advantage + row * in.advantage_row;
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
                 tokens += on[k] ? 1 : 0;
             }
             acc[0] += (double)sum[0];
-            acc[1] += (double)sum[1];
+            if (in.ref) acc[1] += (double)sum[1];
             if (in.entropy) acc[2] += (double)sum[2];
             acc[4] += (double)sum[3];
             if (saved) {
@@ -382,7 +382,7 @@ extern "C" int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t 
         in.high = log1p(clip_high), in.low = log1p(-clip_low);          // clip_low = 1: log 0 = -inf, never below it
         in.far = dual_clip != 0 ? log(dual_clip) : (double)INFINITY;
         in.ratio_high = (float)(1 + clip_high), in.ratio_low = (float)(1 - clip_low), in.ratio_far = (float)dual_clip;
-        in.kl_coef = kl_coef;
+        in.kl_coef = ref_logprob ? kl_coef : 0.f;                       // no KL, no gradient of it
         if (type == kFp32) loss_pick<Single>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
         else if (type == kFp16) loss_pick<Half>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);
         else loss_pick<BFloat16>(in, shape, (float *)saved, (float *)weights, (double *)workspace, s);

@@ -332,3 +332,28 @@ def test_equal_calls_give_equal_bits_and_graphs_replay():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), seed
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,time", [(3, 2), (6, 40), (4, 700), (3, 5000)])
+def test_a_class_of_probability_zero_without_a_reference(dtype, rows, time):
+    """Tokens whose logit the new policy masks (log-probability -inf): their ratio is 0, and without a reference there is
+    no KL to speak of.  Everything but old_kl is what a ratio of e^-200, 0 in fp32, gives."""
+    for per_token in (False, True):
+        data = make(rows, time, dtype, time, ref=False, entropy=False, per_token=per_token)
+        data["mask"] = None
+        gone = torch.zeros(rows, time, dtype=torch.bool, device="cuda")
+        gone[1, time // 2] = gone[2, 0] = gone[0, time - 1] = True
+        outs = []
+        for value in (data["old"].float() - 200, torch.full((rows, time), float("-inf"), device="cuda")):
+            for kl_coef in (0.0, 0.1):
+                leaf = torch.where(gone, value.to(dtype), data["logprob"]).requires_grad_()
+                loss, stats = PolicyLoss(kl_coef=kl_coef)(leaf, data["old"], data["advantages"])
+                outs.append((loss.detach(), stats, torch.autograd.grad(loss, leaf)[0]))
+        for loss, stats, grad in outs:
+            assert torch.equal(loss, outs[0][0]) and torch.equal(stats[:4], outs[0][1][:4]) and torch.equal(grad, outs[0][2])
+            assert torch.isfinite(loss) and torch.isfinite(grad).all() and stats[1] == 0
+        assert outs[-1][1][4] == float("inf")
+        for bad in (float("nan"), float("inf")):
+            stats = PolicyLoss(kl_coef=0.1)(torch.where(gone, bad, data["logprob"]), data["old"], data["advantages"])[1]
+            assert stats[1] == 0 and not torch.isfinite(stats[4])
