@@ -111,7 +111,8 @@ __global__ __launch_bounds__(kPairThreads) void preference_pair_kernel(int64_t p
         const double h = s[0] - s[1], x = beta * h;
         double one = 0, d = 0;
         if (kind == kLogistic) {
-            one = (1.0 - smoothing) * softplus(-x) + smoothing * softplus(x);
+            // a side without weight adds nothing, not 0 * inf: a rejected answer of probability 0 has the margin +inf, the loss 0
+            one = (smoothing < 1.0 ? (1.0 - smoothing) * softplus(-x) : 0.0) + (smoothing > 0.0 ? smoothing * softplus(x) : 0.0);
             d = beta * (smoothing * sigmoid(x) - (1.0 - smoothing) * sigmoid(-x));
         } else if (kind == kSquared) {
             const double off = h - 0.5 / beta;

@@ -191,3 +191,26 @@ def test_equal_bits_and_graph():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), seed
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_margins_without_smoothing(dtype):
+    """A rejected token of probability 0 gives the margin +inf and the loss 0, with its gradient; so does a chosen one
+    under a smoothing of 1.  Everything but the rewards is what a margin far beyond any exponential gives."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    logprob = -torch.rand(8, 30, generator=gen, device="cuda")
+    for smoothing, row in ((0.0, 6), (1.0, 2)):
+        outs = []
+        for value in (-3e4, float("-inf")):
+            x = logprob.clone()
+            x[row, 11] = value
+            leaf = x.to(dtype).requires_grad_()
+            loss, chosen, rejected = PreferenceLoss(beta=0.5, label_smoothing=smoothing)(leaf)
+            outs.append((loss.detach(), torch.autograd.grad(loss, leaf)[0]))
+            assert torch.isfinite(loss) and torch.isfinite(outs[-1][1]).all() and (outs[-1][1][row] == 0).all()
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+        assert torch.cat([chosen, rejected])[row] == float("-inf")
+    for smoothing, row in ((0.1, 6), (0.0, 2), (1.0, 6)):           # here the loss is infinite
+        x = logprob.clone()
+        x[row, 11] = float("-inf")
+        assert PreferenceLoss(label_smoothing=smoothing)(x.to(dtype))[0] == float("inf")
