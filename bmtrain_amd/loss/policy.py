@@ -33,7 +33,9 @@ class PolicyLoss(torch.nn.Module):
     ``ref_logprob`` and ``entropy`` of the same shape and type, ``advantages`` ([sequences], [sequences, 1] or
     [sequences, tokens]) and ``mask`` (non-zero: the token counts; None: all do).  Gradients go to ``logprob`` and
     ``entropy``; the other inputs are constants.  What stands under an unset mask, NaN or infinity included, has no
-    influence, and its gradient is 0.  Sums are held in 64 bits; gradients are rounded once to the inputs' type.
+    influence, and its gradient is 0.  Sums are held in 64 bits; gradients are rounded once to the inputs' type.  A token's
+    own terms are fp32: log-probabilities more than 88 apart make its ratio (or e^q) infinite, which a clip or an advantage
+    of 0 takes away again.
     """
 
     def __init__(self, clip_low: float = 0.2, clip_high: Optional[float] = None, dual_clip: Optional[float] = None,

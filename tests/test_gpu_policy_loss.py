@@ -357,3 +357,28 @@ def test_a_class_of_probability_zero_without_a_reference(dtype, rows, time):
         for bad in (float("nan"), float("inf")):
             stats = PolicyLoss(kl_coef=0.1)(torch.where(gone, bad, data["logprob"]), data["old"], data["advantages"])[1]
             assert stats[1] == 0 and not torch.isfinite(stats[4])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,time", [(3, 2), (6, 40), (4, 700), (3, 5000)])
+def test_no_advantage_and_a_ratio_beyond_fp32(dtype, rows, time):
+    """A token without advantage adds nothing to the policy term and its gradient, however far its ratio is from 1: e^100
+    is infinite in fp32, the product with 0 is not NaN.  Everything but old_kl is what a ratio of e^2 gives."""
+    for per_token in (False, True):
+        data = make(rows, time, dtype, time, per_token=per_token)
+        data["mask"] = None
+        far = torch.zeros(rows, time, dtype=torch.bool, device="cuda")
+        far[1, time // 2] = far[1, 0] = far[1, time - 1] = True
+        data["advantages"] = torch.where(far if per_token else torch.arange(rows, device="cuda") == 1, 0.0, data["advantages"])
+        outs = []
+        for gap in (2.0, 100.0):
+            leaf = data["logprob"].clone().requires_grad_()
+            old = torch.where(far, (data["logprob"].float() - gap).to(dtype), data["old"])
+            loss, stats = PolicyLoss(kl_coef=0.1, reduction="sequence")(leaf, old, data["advantages"], None, data["ref"])
+            outs.append((loss.detach(), stats, torch.autograd.grad(loss, leaf)[0]))
+        (loss, stats, grad), (far_loss, far_stats, far_grad) = outs
+        assert torch.isfinite(far_loss) and torch.isfinite(far_grad).all() and far_stats[4] == float("inf")
+        assert torch.equal(loss, far_loss) and torch.equal(stats[:4], far_stats[:4]) and torch.equal(grad, far_grad)
+        bad = data["logprob"].clone()
+        bad[1, 0] = float("nan")                                    # NaN is no ratio
+        assert torch.isnan(PolicyLoss()(bad, data["old"], data["advantages"])[0])
