@@ -412,7 +412,6 @@ std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const 
         row.src_type = type(g), row.dst_type = type(o);
         expect(g.is_cuda() && g.device() == grads[0].device() && o.device() == g.device(), "gradients must be on one cuda device");
         expect(o.numel() == g.numel(), "outputs must have their gradients' numbers of elements");
-        expect(!g.is_neg() && !o.is_neg(), "gradients must not be lazily negated");
         expect(is_dense(g), "gradients must not have gaps nor elements that share memory");
         expect((g.is_contiguous() && o.is_contiguous()) || (g.sizes() == o.sizes() && g.strides() == o.strides()),
                "outputs must have their gradients' strides");
@@ -426,6 +425,8 @@ Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vec
                   double eps, double scale) {
     const std::vector<Tensor> &outs = outs_in ? *outs_in : grads;
     expect(!grads.empty() && outs.size() == grads.size(), "as many outputs as gradients, at least one");
+    for (const std::vector<Tensor> *list : {&grads, &outs})
+        for (const Tensor &t : *list) expect(!t.is_neg(), "gradients must not be lazily negated");
     const std::vector<bmt_clip_tensor> table = clip_table(grads, outs);
     const int32_t count = (int32_t)table.size();
     const c10::DeviceGuard device(grads[0].device());
@@ -441,7 +442,8 @@ Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vec
     return result.select(0, 0);
 }
 
-// Every gradient times the factor rounded to its type, if the factor (one float on the GPU) is below one.
+// Every gradient times the factor rounded to its type, if the factor (one float on the GPU) is below one.  In place the
+// product rounds alike under either sign, so a lazily negated gradient is scaled in memory as it is.
 void scale_grads(const std::vector<Tensor> &grads, const Tensor &coef) {
     expect(coef.is_cuda() && coef.scalar_type() == at::kFloat && coef.numel() == 1, "coef must be one float on cuda");
     if (grads.empty()) return;

@@ -221,12 +221,12 @@ class OptimManager:
         """`p.grad.mul_(clip_coef)` for every parameter if clip_coef < 1 (optim_manager.py:196-199).  Contiguous GPU
         gradients take one launch per 96 runs of back-to-back ones, which looks at the factor on the GPU: no host read.
         The factor is rounded to each gradient's type there, as torch does with a 0-dim fp32 factor: same bits."""
-        runs = flat_runs([p.grad.data for p in parameters if p.grad is not None])
+        runs = flat_runs([p.grad.data for p in parameters if p.grad is not None and p.grad.numel()])
         fused, rest, end = [], [], 0
         for g in sorted(runs, key=lambda g: g.data_ptr()):
             # a gradient met twice (or one that overlaps another) is scaled twice: one after the other, below
             if (torch.is_tensor(clip_coef) and clip_coef.is_cuda and clip_coef.dtype == torch.float32 and g.is_cuda
-                    and g.device == clip_coef.device and g.is_contiguous() and g.numel() and g.data_ptr() >= end
+                    and g.device == clip_coef.device and g.is_contiguous() and g.data_ptr() >= end
                     and g.dtype in (torch.float16, torch.bfloat16, torch.float32)):
                 fused.append(g)
                 end = g.data_ptr() + g.numel() * g.element_size()

@@ -271,3 +271,27 @@ def test_rounded_factor():
     want = [(g.float() * coef.to(g.dtype).float()).to(g.dtype) for g in grads]
     _tensors.scale_grads(grads, coef)
     assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_manager_scales_negated_and_empty_gradients_without_a_host_read():
+    """A contiguous lazily negated gradient is scaled as its numbers are, an empty one has nothing to scale, and neither
+    makes the host wait for the factor."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for max_norm in (0.01, 1e6):
+            before = grads_of([1000, 1, 77], (dtype,), 8)
+            params = [torch.nn.Parameter(torch.zeros(g.numel(), device="cuda", dtype=dtype)) for g in before]
+            for p, g in zip(params[:2], before):
+                p.grad = torch._neg_view(-g)
+                assert p.grad.is_neg() and torch.equal(p.grad, g)
+            params[2].grad = before[2].clone()
+            empty = torch.nn.Parameter(torch.zeros(0, 3, device="cuda", dtype=dtype))
+            empty.grad = torch.zeros_like(empty)
+            manager = OptimManager(loss_scale=8.0)
+            torch.cuda.set_sync_debug_mode("error")
+            try:
+                norm = manager.clip_grad_norm([{"params": [*params, empty]}], max_norm)
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+            coef = float(max_norm * 8.0) / (norm * 8.0 + 1e-6)
+            for p, g in zip(params, before):
+                assert torch.equal(p.grad, g.mul_(coef) if coef < 1 else g)
