@@ -420,6 +420,13 @@ std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const 
     return table;
 }
 
+// What an in-place operation refuses: where a graph is recorded, a write into a leaf or a view of one would be no part of it.
+void may_be_written(const Tensor &t) {
+    if (!at::GradMode::is_enabled() || !t.requires_grad()) return;
+    TORCH_CHECK(!t.is_leaf() && !(t.is_view() && t._base().is_leaf()),
+                "a leaf that requires a gradient, or a view of one, is written under torch.no_grad() only");
+}
+
 // Clips `grads` into `outs` (None: in place) and returns their norm.
 Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vector<Tensor>> &outs_in, double max_norm, bool use_max,
                   double eps, double scale) {
@@ -427,6 +434,7 @@ Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vec
     expect(!grads.empty() && outs.size() == grads.size(), "as many outputs as gradients, at least one");
     for (const std::vector<Tensor> *list : {&grads, &outs})
         for (const Tensor &t : *list) expect(!t.is_neg(), "gradients must not be lazily negated");
+    for (const Tensor &o : outs) may_be_written(o);
     const std::vector<bmt_clip_tensor> table = clip_table(grads, outs);
     const int32_t count = (int32_t)table.size();
     const c10::DeviceGuard device(grads[0].device());

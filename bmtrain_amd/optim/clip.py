@@ -25,9 +25,10 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type=2.0, ep
         norm_type: 2.0, or ``math.inf`` / ``'inf'`` for the largest magnitude.
         scale: the loss scale the gradients carry; the returned norm is divided by it.
         out: tensors of as many elements as the gradients (of their shapes and strides, where those are not contiguous),
-            of any of the three types, that receive the clipped gradients - fp32 accumulators into the 16-bit gradients of an optimizer, say; ``None``
-            clips in place.  An output may be its own gradient but share memory with nothing else of the call
-            (``RuntimeError``; the gradients themselves are not listed twice either when they are clipped in place).
+            of any of the three types, that receive the clipped gradients - fp32 accumulators into the 16-bit gradients
+            of an optimizer, say; ``None`` clips in place.  An output may be its own gradient but share memory with
+            nothing else of the call (``RuntimeError``; the gradients themselves are not listed twice either when they
+            are clipped in place).  A leaf that requires a gradient is written under ``torch.no_grad()`` only.
 
     Nothing is read by the host, so the call can be captured into a graph.  Squares are summed in 64 bits in a fixed
     order, the product with the factor is fp32 and rounded to the output's type once.  With an infinite norm the factor

@@ -295,3 +295,19 @@ def test_manager_scales_negated_and_empty_gradients_without_a_host_read():
             coef = float(max_norm * 8.0) / (norm * 8.0 + 1e-6)
             for p, g in zip(params, before):
                 assert torch.equal(p.grad, g.mul_(coef) if coef < 1 else g)
+
+
+def test_what_autograd_allows_to_write():
+    """Leaves under no_grad, leaves that are only read, and gradients that carry a graph of their own."""
+    leaf = torch.full((100,), 2.0, device="cuda", requires_grad=True)
+    out = torch.empty(100, device="cuda")
+    check([leaf.detach()], 0.1, out=[out])
+    clip_grads([leaf], 0.1, out=[out])                              # read only
+    want = out.clone()
+    grad, = torch.autograd.grad((leaf ** 3).sum(), leaf, create_graph=True)
+    assert grad.requires_grad
+    clip_grads([grad], 0.1)
+    with torch.no_grad():
+        clip_grads([leaf], 0.1)
+        assert torch.equal(leaf, want)
+        clip_grads([leaf[:50]], 0.01)

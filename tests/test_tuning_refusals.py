@@ -176,3 +176,15 @@ def test_clip_entries():
     with pytest.raises(RuntimeError, match="null"):
         C.grad_norm_multi_launcher(1, address, 0, 1.0, 1e-6, 1.0, 0, 0x2000, 0)
     assert C.grad_norm_workspace_doubles(1, address) == 2 and C.grad_norm_workspace_doubles(0, 0) == 1
+
+
+def test_leaves_are_written_under_no_grad_only():
+    """As with any in-place operation: the write would be no part of the leaf's graph."""
+    for device in ("cpu", "cuda") if torch.cuda.is_available() else ("cpu",):
+        leaf = torch.full((8,), 2.0, device=device, requires_grad=True)
+        plain = torch.full((8,), 2.0, device=device)
+        for call in (lambda: clip_grads([leaf], 0.1), lambda: clip_grads([plain], 0.1, out=[leaf]), lambda: clip_grads([leaf[2:6]], 0.1),
+                     lambda: clip_grads([plain, plain.clone()], 0.1, out=[torch.empty_like(plain), leaf])):
+            with pytest.raises(RuntimeError, match="leaf"):
+                call()
+        assert (leaf == 2).all() and (plain == 2).all()
