@@ -399,6 +399,8 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor &logprob_in, con
 // True if the elements fill one run of memory without gaps, in whatever order of dimensions.
 bool is_dense(const Tensor &t) { return t.numel() == 0 || t.is_non_overlapping_and_dense(); }
 
+// SIGNS: a lazily negated gradient or output is refused.
+template <bool SIGNS>
 std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const std::vector<Tensor> &outs) {
     std::vector<bmt_clip_tensor> table(grads.size());
     auto type = [](const Tensor &t) {
@@ -412,6 +414,7 @@ std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const 
         row.src_type = type(g), row.dst_type = type(o);
         expect(g.is_cuda() && g.device() == grads[0].device() && o.device() == g.device(), "gradients must be on one cuda device");
         expect(o.numel() == g.numel(), "outputs must have their gradients' numbers of elements");
+        expect(!SIGNS || (!g.is_neg() && !o.is_neg()), "gradients must not be lazily negated");
         expect(is_dense(g), "gradients must not have gaps nor elements that share memory");
         expect((g.is_contiguous() && o.is_contiguous()) || (g.sizes() == o.sizes() && g.strides() == o.strides()),
                "outputs must have their gradients' strides");
@@ -420,10 +423,9 @@ std::vector<bmt_clip_tensor> clip_table(const std::vector<Tensor> &grads, const 
     return table;
 }
 
-// What an in-place operation refuses: where a graph is recorded, a write into a leaf or a view of one would be no part of it.
+// What an in-place operation refuses where a graph is recorded: a write into a leaf or a view of one would be no part of it.
 void may_be_written(const Tensor &t) {
-    if (!at::GradMode::is_enabled() || !t.requires_grad()) return;
-    TORCH_CHECK(!t.is_leaf() && !(t.is_view() && t._base().is_leaf()),
+    TORCH_CHECK(!t.requires_grad() || (!t.is_leaf() && !(t.is_view() && t._base().is_leaf())),
                 "a leaf that requires a gradient, or a view of one, is written under torch.no_grad() only");
 }
 
@@ -432,10 +434,9 @@ Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vec
                   double eps, double scale) {
     const std::vector<Tensor> &outs = outs_in ? *outs_in : grads;
     expect(!grads.empty() && outs.size() == grads.size(), "as many outputs as gradients, at least one");
-    for (const std::vector<Tensor> *list : {&grads, &outs})
-        for (const Tensor &t : *list) expect(!t.is_neg(), "gradients must not be lazily negated");
-    for (const Tensor &o : outs) may_be_written(o);
-    const std::vector<bmt_clip_tensor> table = clip_table(grads, outs);
+    if (at::GradMode::is_enabled())
+        for (const Tensor &o : outs) may_be_written(o);
+    const std::vector<bmt_clip_tensor> table = clip_table<true>(grads, outs);
     const int32_t count = (int32_t)table.size();
     const c10::DeviceGuard device(grads[0].device());
     const Tensor result = floats({2}, grads[0]);
@@ -455,7 +456,7 @@ Tensor clip_grads(const std::vector<Tensor> &grads, const std::optional<std::vec
 void scale_grads(const std::vector<Tensor> &grads, const Tensor &coef) {
     expect(coef.is_cuda() && coef.scalar_type() == at::kFloat && coef.numel() == 1, "coef must be one float on cuda");
     if (grads.empty()) return;
-    const std::vector<bmt_clip_tensor> table = clip_table(grads, grads);
+    const std::vector<bmt_clip_tensor> table = clip_table<false>(grads, grads);
     expect(grads[0].device() == coef.device(), "gradients and coef must be on one cuda device");
     const c10::DeviceGuard device(coef.device());
     launched("grad_scale_multi_launcher",
