@@ -30,7 +30,7 @@ class OpFusedCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output: torch.Tensor):
-        grad_output = grad_output.contiguous()
+        grad_output = grad_output.resolve_neg().contiguous()        # the kernel reads the memory: no lazily negated view
         softmax, target = ctx.saved_tensors
         F.cross_entropy_backward_inplace(softmax.size(0), softmax.size(1), grad_output, target, softmax,
                                          ctx.ignore_index)
@@ -60,7 +60,7 @@ class OpLossReduce(torch.autograd.Function):
     def backward(ctx, upstream: torch.Tensor):
         target, weight_sum, weight = ctx.saved_tensors
         n_classes, ignore_index, mean = ctx.args
-        upstream = upstream.float().contiguous()
+        upstream = upstream.float().resolve_neg().contiguous()
         grad_rows = torch.empty(target.numel(), device=target.device, dtype=torch.float)
         F.loss_reduce_backward(target, weight, n_classes, ignore_index, mean, weight_sum, upstream, grad_rows)
         return (grad_rows, None, None, None, None, None)

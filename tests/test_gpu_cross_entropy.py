@@ -620,3 +620,23 @@ def test_more_than_2_to_the_31_logits():
     assert np.array_equal(bits16(softmax[idx]), want)
     del x, softmax
     torch.cuda.empty_cache()
+
+
+def test_lazily_negated_upstreams():
+    """Complex arithmetic behind a loss hands back upstream gradients whose numbers are the memory's, negated."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    logits = torch.randn(9, 300, generator=gen, device="cuda").half()
+    target = torch.randint(0, 300, (9,), generator=gen, device="cuda")
+    zero = torch.zeros((), device="cuda")
+    for reduction in ("mean", "sum"):
+        loss_func = FusedCrossEntropy(reduction=reduction)
+        x = logits.clone().requires_grad_()
+        want, = torch.autograd.grad(loss_func(x, target), x)
+        (torch.complex(zero, loss_func(x, target)).conj() * (1 + 2j)).imag.backward()          # the loss's share of it is -1
+        assert torch.equal(x.grad, -want), reduction
+    x = logits.clone().requires_grad_()
+    rows = OpFusedCrossEntropy.apply(x, target.int(), -100)
+    g = torch.rand(9, generator=gen, device="cuda")
+    want, = torch.autograd.grad(rows, x, -g)
+    rows = OpFusedCrossEntropy.apply(x, target.int(), -100)
+    assert torch.equal(torch.autograd.grad(rows, x, torch._neg_view(g))[0], want)
