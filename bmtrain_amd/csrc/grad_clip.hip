@@ -194,7 +194,8 @@ __device__ __forceinline__ void scale_tile(const void *src, void *dst, int64_t n
 }
 
 template <typename S>
-__device__ __forceinline__ void scale_tile_into(int dst_type, const void *src, void *dst, int64_t n, int64_t number, float c, int32_t round_coef) {
+__device__ __forceinline__ void scale_tile_into(int dst_type, const void *src, void *dst, int64_t n, int64_t number, float c,
+                                                int32_t round_coef) {
     if (dst_type == kFp32) scale_tile<S, Single>(src, dst, n, number, c, round_coef);
     else if (dst_type == kFp16) scale_tile<S, Half>(src, dst, n, number, c, round_coef);
     else scale_tile<S, BFloat16>(src, dst, n, number, c, round_coef);
@@ -345,9 +346,11 @@ extern "C" int grad_norm_multi_launcher(int32_t count, const bmt_clip_tensor *te
     });
     if (e != hipSuccess) return fail((int)e, who, e);
     if (use_max)
-        hipLaunchKernelGGL((grad_norm_finish_kernel<true>), dim3(1), dim3(kThreads), 0, s, partials, used, max_norm, eps, scale, (float *)out);
+        hipLaunchKernelGGL((grad_norm_finish_kernel<true>), dim3(1), dim3(kThreads), 0, s, partials, used, max_norm, eps, scale,
+                           (float *)out);
     else
-        hipLaunchKernelGGL((grad_norm_finish_kernel<false>), dim3(1), dim3(kThreads), 0, s, partials, used, max_norm, eps, scale, (float *)out);
+        hipLaunchKernelGGL((grad_norm_finish_kernel<false>), dim3(1), dim3(kThreads), 0, s, partials, used, max_norm, eps, scale,
+                           (float *)out);
     e = hipGetLastError();
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }
@@ -367,7 +370,8 @@ extern "C" int grad_scale_multi_launcher(int32_t count, const bmt_clip_tensor *t
     }
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = in_batches(count, tensors, kScaleTile, kScaleThreads, true, [&](const Batch &b, uint32_t tiles, int types) {
-        scale_launch(std::integer_sequence<int, kMixed, 0, 1, 2, 4, 5, 6, 8, 9, 10>(), b, tiles, types, (const float *)coef, round_coef, s);
+        scale_launch(std::integer_sequence<int, kMixed, 0, 1, 2, 4, 5, 6, 8, 9, 10>(), b, tiles, types, (const float *)coef,
+                     round_coef, s);
     });
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }

@@ -90,8 +90,8 @@ __device__ __forceinline__ void workgroup_sums(double *v, double (*slots)[8], do
     __syncthreads();
 }
 
-// COL: one advantage for each token, not one for a row.  kWhole: the workgroup's lanes work on one unit; kGroups: groups of in.lanes lanes of a wave do; kTiny: the same for rows of
-// up to three tokens.
+// COL: one advantage for each token, not one for a row.  kWhole: the workgroup's lanes work on one unit; kGroups: groups of
+// in.lanes lanes of a wave do; kTiny: the same for rows of up to three tokens.
 enum Form { kWhole, kGroups, kTiny };
 template <typename T, Form FORM, bool COL>
 __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, uint32_t units, float *__restrict__ saved,
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
         const int end = there ? (in.time - begin < in.unit ? in.time : begin + in.unit) : 0;
         const Bits *lp = (const Bits *)in.logprob + row * in.logprob_row;
         const Bits *op = (const Bits *)in.old + row * in.old_row;
-        const Bits *fp = in.ref ? (const Bits *)in.ref + row * in.ref_row : lp;      // absent: q is 0, or NaN where l is not finite, and not used
+        // without a reference q is 0, or NaN where l is not finite, and not used
+        const Bits *fp = in.ref ? (const Bits *)in.ref + row * in.ref_row : lp;
         const Bits *ep = (const Bits *)in.entropy + row * in.entropy_row;
         const uint8_t *mp = in.mask ? in.mask + row * in.mask_row : nullptr;
         const float *ap = in.advantage + row * in.advantage_row;
@@ -259,7 +260,8 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
         const double share = reduction == kSum ? 1.0 : all[5] > 0 ? 1.0 / all[5] : 0.0;     // nothing counts: loss 0
         for (int k = 0; k < 5; k++) all[k] *= share;
         // a term without weight is only measured: no 0 * inf
-        loss[0] = (float)(all[0] + (kl_coef != 0.f ? (double)kl_coef * all[1] : 0.0) - (entropy_coef != 0.f ? (double)entropy_coef * all[2] : 0.0));
+        loss[0] = (float)(all[0] + (kl_coef != 0.f ? (double)kl_coef * all[1] : 0.0) -
+                          (entropy_coef != 0.f ? (double)entropy_coef * all[2] : 0.0));
         for (int k = 0; k < 5; k++) stats[k] = (float)all[k];
         weights[0] = (float)share;
     }
@@ -381,7 +383,8 @@ extern "C" int policy_loss_forward_launcher(int64_t rows, int64_t time, int32_t 
         in.advantage = (const float *)advantage, in.mask = (const uint8_t *)mask;
         in.logprob_row = logprob_row, in.old_row = old_row, in.ref_row = ref_row, in.entropy_row = entropy_row;
         in.advantage_row = advantage_row, in.mask_row = mask_row, in.advantage_col = advantage_col;
-        in.rows = (int32_t)rows, in.time = (int32_t)time, in.chunks = shape.chunks, in.unit = shape.unit, in.lanes = shape.lanes, in.reduction = reduction;
+        in.rows = (int32_t)rows, in.time = (int32_t)time, in.reduction = reduction;
+        in.chunks = shape.chunks, in.unit = shape.unit, in.lanes = shape.lanes;
         in.high = log1p(clip_high), in.low = log1p(-clip_low);          // clip_low = 1: log 0 = -inf, never below it
         in.far = dual_clip != 0 ? log(dual_clip) : (double)INFINITY;
         in.ratio_high = (float)(1 + clip_high), in.ratio_low = (float)(1 - clip_low), in.ratio_far = (float)dual_clip;

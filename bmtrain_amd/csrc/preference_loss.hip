@@ -11,7 +11,8 @@
 // Back: dl[i, t] = +-m (dloss/dh) / pairs (/ n_i), the sign that of the row.
 // h is a small difference of large sums, so the sums and everything per pair are held in 64 bits.
 //
-// A unit is a row's part of up to 1,024 tokens (4,096 in large batches; 8, 64 or 256 lanes); one workgroup turns the units' sums into pairs.
+// A unit is a row's part of up to 1,024 tokens (4,096 in large batches; 8, 64 or 256 lanes); one workgroup turns the units'
+// sums into pairs.
 // Bound by HBM for large batches (fp32: 9 B read per token forward, 1 read and 4 written back), by launches for small.
 #include "bmt_vec.h"
 #include "../../include/bmt_hip.h"
@@ -177,9 +178,9 @@ void sum_launch(int64_t rows, int64_t time, const void *logprob, int64_t logprob
                 const void *mask, int64_t mask_row, RowSum *sums, hipStream_t s) {
     const int64_t chunks = chunks_of(rows / 2, time), units = rows * chunks, groups = kThreads / LANES;
     typedef typename Elem<T>::Bits Bits;
-    hipLaunchKernelGGL((preference_sum_kernel<T, LANES>), dim3((unsigned)((units + groups - 1) / groups)), dim3(kThreads), 0, s, units,
-                       (int32_t)chunks, (int32_t)part_of(rows / 2, time), (int32_t)time, (const Bits *)logprob, logprob_row, (const Bits *)ref, ref_row,
-                       (const uint8_t *)mask, mask_row, sums);
+    hipLaunchKernelGGL((preference_sum_kernel<T, LANES>), dim3((unsigned)((units + groups - 1) / groups)), dim3(kThreads), 0, s,
+                       units, (int32_t)chunks, (int32_t)part_of(rows / 2, time), (int32_t)time, (const Bits *)logprob, logprob_row,
+                       (const Bits *)ref, ref_row, (const uint8_t *)mask, mask_row, sums);
 }
 template <typename T>
 void sum_pick(int64_t rows, int64_t time, const void *logprob, int64_t logprob_row, const void *ref, int64_t ref_row,
@@ -211,7 +212,8 @@ extern "C" int preference_loss_forward_launcher(int64_t pairs, int64_t time, int
     if (!(beta > 0) || !(beta <= 1e30)) return refuse(who, "beta must be positive and finite");
     if (!(label_smoothing >= 0 && label_smoothing <= 1)) return refuse(who, "label_smoothing must be in [0, 1]");
     if (!fits(pairs, time)) return refuse(who, "too many tokens for one launch");
-    if (!loss || !workspace || !slope || (pairs > 0 && (!chosen || !rejected || (time > 0 && !logprob)))) return refuse(who, "null pointer");
+    if (!loss || !workspace || !slope || (pairs > 0 && (!chosen || !rejected || (time > 0 && !logprob))))
+        return refuse(who, "null pointer");
     if ((uintptr_t)workspace % 8 || ((uintptr_t)loss | (uintptr_t)chosen | (uintptr_t)rejected | (uintptr_t)slope) % 4)
         return refuse(who, "misaligned output");
     if (((uintptr_t)logprob | (uintptr_t)ref_logprob) % (type == kFp32 ? 4 : 2)) return refuse(who, "misaligned input");
@@ -224,8 +226,8 @@ extern "C" int preference_loss_forward_launcher(int64_t pairs, int64_t time, int
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return fail((int)e, who, e);
     }
-    hipLaunchKernelGGL(preference_pair_kernel, dim3(1), dim3(kPairThreads), 0, s, pairs, (int32_t)chunks_of(pairs, time), sums, kind, average,
-                       beta, label_smoothing, (float *)loss, (float *)chosen, (float *)rejected, (float *)slope);
+    hipLaunchKernelGGL(preference_pair_kernel, dim3(1), dim3(kPairThreads), 0, s, pairs, (int32_t)chunks_of(pairs, time), sums,
+                       kind, average, beta, label_smoothing, (float *)loss, (float *)chosen, (float *)rejected, (float *)slope);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail((int)e, who, e);
 }

@@ -481,7 +481,7 @@ PYBIND11_MODULE(_tensors, m) {
     m.def("preference_loss", wrap_pybind_function_no_gil(preference_loss), py::arg("logprob"), py::arg("ref_logprob"), py::arg("mask"),
           py::arg("kind"), py::arg("average"), py::arg("beta"), py::arg("label_smoothing"));
     m.def("is_dense", wrap_pybind_function_no_gil(is_dense));
-    m.def("clip_grads", wrap_pybind_function_no_gil(clip_grads), py::arg("grads"), py::arg("outs"), py::arg("max_norm"), py::arg("use_max"),
-          py::arg("eps"), py::arg("scale"));
+    m.def("clip_grads", wrap_pybind_function_no_gil(clip_grads), py::arg("grads"), py::arg("outs"), py::arg("max_norm"),
+          py::arg("use_max"), py::arg("eps"), py::arg("scale"));
     m.def("scale_grads", wrap_pybind_function_no_gil(scale_grads), py::arg("grads"), py::arg("coef"));
 }

@@ -302,8 +302,8 @@ __global__ __launch_bounds__(ROW < 256 ? 256 : ROW) void token_logprobs_backward
 // Rows of up to this many elements go one to a wave: a workgroup's meeting point and its idle lanes cost more there.
 constexpr int32_t kWaveRow = 4096;
 
-static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void *x, int32_t type, const void *target, int32_t target_bits,
-                              float temperature) {
+static const char *check_rows(int64_t rows, int64_t inner, int64_t n, const void *x, int32_t type, const void *target,
+                              int32_t target_bits, float temperature) {
     if (type != kFp32 && type != kFp16 && type != kBf16) return "unknown type code";
     if (rows > 0x7FFFFFFF || n > 0x7FFFFFF0 || inner > 0x7FFFFFFF || inner < 1) return "too many rows or classes";
     if (!x || !target) return "null pointer";
@@ -321,8 +321,8 @@ static const char *forward_launch(const LogitRows &in, const Targets &t, float i
     constexpr int PER = ROW < 256 ? 256 / ROW : 1;
     const unsigned grid = (unsigned)((in.rows + (int64_t)PER - 1) / PER);
     if (!launch_fits(grid, ROW < 256 ? 256 : ROW)) return "too many rows for one launch";
-    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY, PAST>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream, in, t, inv_t,
-                       logprob, entropy, stats);
+    hipLaunchKernelGGL((token_logprobs_kernel<T, ROW, UNROLL, ENTROPY, PAST>), dim3(grid), dim3(ROW < 256 ? 256 : ROW), 0, stream,
+                       in, t, inv_t, logprob, entropy, stats);
     return nullptr;
 }
 // Logits of up to this many bytes go through the caches on the way forward: what the 256 MiB of the last level keep of
@@ -363,11 +363,11 @@ static const char *backward_launch(const LogitRows &in, const Targets &t, float 
     if (in.rows * tiles > 0x7FFFFFFF || !launch_fits(grid, threads)) return "too many elements for one launch";
     typedef typename Elem<T>::Bits Bits;
     if (ge)
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(threads), 0, stream, in, t, inv_t,
-                           stats, gl, ge, (Bits *)grad, (int32_t)tiles);
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, true>), dim3((unsigned)grid), dim3(threads), 0, stream,
+                           in, t, inv_t, stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     else
-        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, false>), dim3((unsigned)grid), dim3(threads), 0, stream, in, t, inv_t,
-                           stats, gl, ge, (Bits *)grad, (int32_t)tiles);
+        hipLaunchKernelGGL((token_logprobs_backward_kernel<T, ROW, UNROLL, false>), dim3((unsigned)grid), dim3(threads), 0, stream,
+                           in, t, inv_t, stats, gl, ge, (Bits *)grad, (int32_t)tiles);
     return nullptr;
 }
 template <typename T>

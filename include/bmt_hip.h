@@ -287,7 +287,8 @@ BMT_API int grad_stats_multi_launcher(int32_t count, const bmt_scan_tensor *tens
  *   logprob[r] = z_target - L;   entropy[r] = L - sum_j e^z_j z_j / sum_j e^z_j   (fp32; entropy may be NULL)
  *   stats: float[4 * rows] for the backward call, or NULL;
  *   grad[r, j] = (g (1[j == target] - p_j) - h p_j (log p_j + entropy[r])) / T,  p_j = e^(z_j - L), contiguous [rows, n]
- * with g = grad_logprob[r], h = grad_entropy[r] (fp32; either may be NULL for zeros).
+ * with g = grad_logprob[r], h = grad_entropy[r] (fp32; either may be NULL for zeros; grad_entropy needs the stats of a
+ * forward call that was asked for the entropy).
  * A row whose target is ignore_index has results 0 and a gradient row of 0, and its logits are not read; a row with
  * g == h == 0 has a gradient row of 0 and is not read on the way back.  Another target outside [0, n): logprob NaN, and
  * a gradient without the one-hot term.
@@ -307,6 +308,7 @@ BMT_API int token_logprobs_backward_launcher(int64_t rows, int64_t n, int64_t in
  *   policy = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), and at most -dual_clip A where A < 0 (dual_clip 0: none)
  *   kl = e^q - 1 - q (0 without ref),   old_kl = e^d - 1 - d
  *   loss = R(policy) + kl_coef R(kl) - entropy_coef R(entropy);   stats[5] = R of policy, kl, entropy, clipped, old_kl
+ * A token's terms are fp32: r and e^q are infinite from 2^128 on (r times an advantage of 0 is 0 then, too).
  * reduction 0: mean over the tokens under the mask; 1: mean over the sequences with tokens of their means; 2: sum.
  * Nothing under the mask: 0.  advantage: float, one per row (advantage_col 0) or per token (1).
  * saved: float[rows * time] (the derivative before its weight) or NULL when no backward call follows; weights:
