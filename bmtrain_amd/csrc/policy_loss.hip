@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(PolicyIn in, 
                     under = A[k] < 0.f && wide < in.low;
                     if (!(fabsf(d[k]) < 1.f)) {
                         rm1 = expf(d[k]) - 1.f, old_kl = rm1 - d[k];
-                        if (A[k] == 0.f && rm1 == INFINITY && d[k] < INFINITY) rm1 = 0.f;      // e^d beyond fp32 times 0 is 0, not NaN
+                        if (A[k] == 0.f && rm1 == INFINITY) rm1 = 0.f;      // e^d beyond fp32 times 0 is 0, not NaN
                     }
                     if (!(fabsf(q[k]) < 1.f)) qm1 = expf(q[k]) - 1.f, kl = qm1 - q[k];
                 }

@@ -379,6 +379,10 @@ def test_no_advantage_and_a_ratio_beyond_fp32(dtype, rows, time):
         (loss, stats, grad), (far_loss, far_stats, far_grad) = outs
         assert torch.isfinite(far_loss) and torch.isfinite(far_grad).all() and far_stats[4] == float("inf")
         assert torch.equal(loss, far_loss) and torch.equal(stats[:4], far_stats[:4]) and torch.equal(grad, far_grad)
+        old = torch.where(far, float("-inf"), data["old"])          # what the old policy could not have sampled
+        gone, gone_stats = PolicyLoss(kl_coef=0.1, reduction="sequence")(leaf, old, data["advantages"], None, data["ref"])
+        assert torch.equal(loss, gone) and torch.equal(stats[:4], gone_stats[:4])
+        assert torch.equal(grad, torch.autograd.grad(gone, leaf)[0])
         bad = data["logprob"].clone()
         bad[1, 0] = float("nan")                                    # NaN is no ratio
         assert torch.isnan(PolicyLoss()(bad, data["old"], data["advantages"])[0])
